@@ -294,6 +294,174 @@ void v1_chunk_attention(const at::Tensor& query, const at::Tensor& kv_cache, con
       rotation.has_value() ? rotation->data_ptr<float>() : nullptr, stream_of(query)));
 }
 
+void v1_tree_attention(const at::Tensor& query, const at::Tensor& kv_cache, const at::Tensor& block_table,
+                       const at::Tensor& seq_lens, const at::Tensor& query_start_loc,
+                       const std::optional<at::Tensor>& tree_mask, const std::optional<at::Tensor>& kv_start,
+                       const std::optional<at::Tensor>& centroids, int64_t key_bits, int64_t value_bits, double scale,
+                       int64_t v_flags, int64_t max_query_len, int64_t num_splits, at::Tensor& workspace, at::Tensor& out,
+                       std::optional<at::Tensor> lse, const std::optional<at::Tensor>& rotation) {
+  contig(query, "query");
+  on_device(kv_cache, "kv_cache");
+  contig(block_table, "block_table");
+  contig(seq_lens, "seq_lens");
+  contig(query_start_loc, "query_start_loc");
+  contig(workspace, "workspace");
+  contig(out, "out");
+  TORCH_CHECK(query.dim() == 3 && out.sizes() == query.sizes(), "fused_tq: query and out must be [T, Hq, d]");
+  TORCH_CHECK(kv_cache.dim() == 4 && kv_cache.scalar_type() == at::kByte && kv_cache.stride(3) == 1,
+              "fused_tq: kv_cache must be uint8 [num_blocks, block_size, Hkv, slot] with contiguous slots");
+  const int64_t T = query.size(0), B = seq_lens.numel(), hq = query.size(1), d = query.size(2);
+  TORCH_CHECK(block_table.scalar_type() == at::kInt && seq_lens.scalar_type() == at::kInt &&
+                  query_start_loc.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == B &&
+                  query_start_loc.numel() == B + 1,
+              "fused_tq: block_table must be int32 [B, max_blocks], seq_lens [B] and query_start_loc [B + 1]");
+  if (tree_mask.has_value()) {
+    contig(*tree_mask, "tree_mask");
+    TORCH_CHECK(tree_mask->scalar_type() == at::kLong && tree_mask->dim() == 2 && tree_mask->size(0) == T,
+                "fused_tq: tree_mask must be int64 [T, words]");
+  }
+  if (kv_start.has_value()) {
+    contig(*kv_start, "kv_start");
+    TORCH_CHECK(kv_start->scalar_type() == at::kInt && kv_start->numel() == T, "fused_tq: kv_start must be int32 [T]");
+  }
+  if (lse.has_value()) {
+    contig(*lse, "lse");
+    TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->numel() == T * hq, "fused_tq: lse must be float32 [T, Hq]");
+  }
+  // the kernels read 2^key_bits centroids and a d x d rotation (raw slots and fp8 keys: no centroids)
+  if (centroids.has_value()) {
+    contig(*centroids, "centroids");
+    TORCH_CHECK_VALUE(centroids->scalar_type() == at::kFloat && (key_bits < 1 || key_bits > 8 || (v_flags & 4) != 0 ||
+                                                                 centroids->numel() == ((int64_t)1 << key_bits)),
+                      "fused_tq: centroids must be float32 with 2^key_bits entries");
+  }
+  if (rotation.has_value()) {
+    contig(*rotation, "rotation");
+    TORCH_CHECK_VALUE(rotation->scalar_type() == at::kFloat && rotation->numel() == d * d, "fused_tq: rotation must be float32 [d, d]");
+  }
+  TORCH_CHECK_VALUE(T <= INT32_MAX && B <= INT32_MAX && block_table.size(1) <= INT32_MAX && max_query_len >= 0 &&
+                        max_query_len <= INT32_MAX && num_splits >= 0 && num_splits <= INT32_MAX,
+                    "fused_tq: token / sequence / split counts out of range");
+  const c10::DeviceGuard g(query.device());
+  check_rc(ftq_v1_tree_attention(
+      query.data_ptr(), dt(query), T, kv_cache.data_ptr<uint8_t>(), kv_cache.size(0), (int)kv_cache.size(1),
+      kv_cache.stride(0), kv_cache.stride(1), kv_cache.stride(2), block_table.data_ptr<int32_t>(), (int)block_table.size(1),
+      seq_lens.data_ptr<int32_t>(), query_start_loc.data_ptr<int32_t>(),
+      tree_mask.has_value() ? reinterpret_cast<const uint64_t*>(tree_mask->data_ptr<int64_t>()) : nullptr,
+      tree_mask.has_value() ? (int)tree_mask->size(1) : 0, kv_start.has_value() ? kv_start->data_ptr<int32_t>() : nullptr,
+      (int)B, (int)max_query_len, (int)hq, (int)kv_cache.size(2), (int)d,
+      centroids.has_value() ? centroids->data_ptr<float>() : nullptr, (int)key_bits, (int)value_bits, (float)scale,
+      (int)v_flags, (int)num_splits, workspace.data_ptr(), workspace.numel() * workspace.element_size(), out.data_ptr(),
+      dt(out), lse.has_value() ? lse->data_ptr<float>() : nullptr,
+      rotation.has_value() ? rotation->data_ptr<float>() : nullptr, stream_of(query)));
+}
+
+// ---- steps of a speculative decode ----
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> step_tables(
+    const at::Tensor& query_start_loc, const at::Tensor& past_lens, const std::optional<at::Tensor>& depths,
+    at::Tensor block_table, int64_t block_size, int64_t num_tokens, std::optional<at::Tensor> num_blocks,
+    std::optional<at::Tensor> free_blocks, std::optional<at::Tensor> free_count) {
+  contig(query_start_loc, "query_start_loc");
+  contig(past_lens, "past_lens");
+  on_device(block_table, "block_table");
+  const int64_t B = past_lens.numel();
+  TORCH_CHECK(query_start_loc.scalar_type() == at::kInt && past_lens.scalar_type() == at::kInt &&
+                  query_start_loc.numel() == B + 1,
+              "fused_tq: query_start_loc must be int32 [B + 1] and past_lens int32 [B]");
+  TORCH_CHECK(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == B &&
+                  (block_table.size(1) <= 1 || block_table.stride(1) == 1) &&
+                  (B <= 1 || block_table.stride(0) >= block_table.size(1)),
+              "fused_tq: block_table must be int32 [B, max_blocks] with contiguous rows");
+  TORCH_CHECK_VALUE(num_tokens >= 0 && block_size >= 1 && block_size <= INT32_MAX && block_table.size(1) <= INT32_MAX &&
+                        B <= INT32_MAX,
+                    "fused_tq: num_tokens / block_size / max_blocks out of range");
+  if (depths.has_value()) {
+    contig(*depths, "depths");
+    TORCH_CHECK(depths->scalar_type() == at::kInt && depths->numel() >= num_tokens, "fused_tq: depths must be int32 [num_tokens]");
+  }
+  const bool alloc = num_blocks.has_value();
+  TORCH_CHECK(free_blocks.has_value() == alloc && free_count.has_value() == alloc,
+              "fused_tq: num_blocks, free_blocks and free_count go together");
+  if (alloc) {
+    for (const at::Tensor* t : {&*num_blocks, &*free_blocks, &*free_count}) {
+      contig(*t, "num_blocks, free_blocks and free_count");
+      TORCH_CHECK(t->scalar_type() == at::kInt, "fused_tq: num_blocks, free_blocks and free_count must be int32");
+    }
+    TORCH_CHECK(num_blocks->numel() == B && free_count->numel() == 1 && free_blocks->numel() <= INT32_MAX,
+                "fused_tq: num_blocks must be [B] and free_count [1]");
+  }
+  const c10::DeviceGuard g(past_lens.device());
+  const auto i32 = past_lens.options();
+  at::Tensor slots = at::empty({num_tokens}, i32.dtype(at::kLong)), pos = at::empty({num_tokens}, i32.dtype(at::kLong));
+  at::Tensor req = at::empty({num_tokens}, i32), lens = at::empty({B}, i32), missing = at::empty({1}, i32);
+  check_rc(ftq_step_tables(query_start_loc.data_ptr<int32_t>(), past_lens.data_ptr<int32_t>(),
+                           depths.has_value() ? depths->data_ptr<int32_t>() : nullptr, (int)B, num_tokens,
+                           block_table.data_ptr<int32_t>(), B > 1 ? block_table.stride(0) : block_table.size(1),
+                           (int)block_table.size(1), (int)block_size, alloc ? num_blocks->data_ptr<int32_t>() : nullptr,
+                           alloc ? free_blocks->data_ptr<int32_t>() : nullptr, alloc ? free_count->data_ptr<int32_t>() : nullptr,
+                           alloc ? (int)free_blocks->numel() : 0, slots.data_ptr<int64_t>(), pos.data_ptr<int64_t>(),
+                           req.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), missing.data_ptr<int32_t>(),
+                           stream_of(past_lens)));
+  return {slots, pos, req, lens, missing};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> tree_accept(const at::Tensor& tokens, const at::Tensor& parents,
+                                                           const at::Tensor& targets, const at::Tensor& query_start_loc,
+                                                           int64_t max_nodes) {
+  contig(tokens, "tokens");
+  contig(parents, "parents");
+  contig(targets, "targets");
+  contig(query_start_loc, "query_start_loc");
+  TORCH_CHECK(tokens.scalar_type() == at::kLong && targets.scalar_type() == at::kLong && parents.scalar_type() == at::kInt &&
+                  query_start_loc.scalar_type() == at::kInt && tokens.numel() == targets.numel() &&
+                  tokens.numel() == parents.numel() && query_start_loc.numel() >= 1,
+              "fused_tq: tokens and targets must be int64, parents int32, one entry per node; query_start_loc int32 [B + 1]");
+  TORCH_CHECK_VALUE(max_nodes >= 1 && max_nodes <= 2048 && query_start_loc.numel() <= INT32_MAX,
+                    "fused_tq: max_nodes must be in [1, 2048]");
+  const c10::DeviceGuard g(query_start_loc.device());
+  const int64_t B = query_start_loc.numel() - 1;
+  at::Tensor path = at::empty({B, max_nodes}, parents.options()), counts = at::empty({B}, parents.options());
+  at::Tensor out = at::empty({B, max_nodes}, tokens.options());
+  check_rc(ftq_tree_accept(tokens.data_ptr<int64_t>(), parents.data_ptr<int32_t>(), targets.data_ptr<int64_t>(),
+                           query_start_loc.data_ptr<int32_t>(), (int)B, tokens.numel(), (int)max_nodes,
+                           path.data_ptr<int32_t>(), counts.data_ptr<int32_t>(), out.data_ptr<int64_t>(),
+                           stream_of(query_start_loc)));
+  return {path, counts, out};
+}
+
+void commit_slots(at::TensorList kv_caches, const at::Tensor& block_table, const at::Tensor& past_lens,
+                  const at::Tensor& path, const at::Tensor& counts) {
+  contig(block_table, "block_table");
+  contig(past_lens, "past_lens");
+  contig(path, "path");
+  contig(counts, "counts");
+  if (kv_caches.empty()) return;
+  const at::Tensor& c0 = kv_caches[0];
+  std::vector<uint8_t*> ptrs;
+  for (const at::Tensor& c : kv_caches) {
+    on_device(c, "kv_cache");
+    TORCH_CHECK(c.dim() == 4 && c.scalar_type() == at::kByte && c.stride(3) == 1 && c.sizes() == c0.sizes() &&
+                    c.strides() == c0.strides() && c.device() == block_table.device(),
+                "fused_tq: kv_caches must be uint8 [num_blocks, block_size, Hkv, slot] of one shape, layout and device");
+    ptrs.push_back(c.data_ptr<uint8_t>());
+  }
+  const int64_t B = block_table.dim() == 2 ? block_table.size(0) : -1;
+  TORCH_CHECK(B >= 0 && block_table.scalar_type() == at::kInt && past_lens.scalar_type() == at::kInt &&
+                  path.scalar_type() == at::kInt && counts.scalar_type() == at::kInt && past_lens.numel() == B &&
+                  counts.numel() == B && path.dim() == 2 && path.size(0) == B,
+              "fused_tq: block_table must be int32 [B, max_blocks], past_lens and counts int32 [B], path int32 [B, n]");
+  TORCH_CHECK_VALUE(B <= INT32_MAX && block_table.size(1) <= INT32_MAX && path.size(1) <= INT32_MAX &&
+                        c0.size(1) <= INT32_MAX && c0.size(3) <= INT32_MAX,
+                    "fused_tq: commit_slots sizes out of range");
+  const c10::DeviceGuard g(block_table.device());
+  check_rc(ftq_commit_slots(ptrs.data(), (int)ptrs.size(), c0.size(0), (int)c0.size(1), c0.stride(0), c0.stride(1),
+                            c0.stride(2), (int)c0.size(2), (int)c0.size(3), block_table.data_ptr<int32_t>(),
+                            block_table.size(1), (int)block_table.size(1), past_lens.data_ptr<int32_t>(),
+                            path.data_ptr<int32_t>(), counts.data_ptr<int32_t>(), (int)path.size(1), (int)B,
+                            stream_of(block_table)));
+}
+
 // ---- library-format attention: windows, other head dims, several tokens ----
 
 void lib_attention(const at::Tensor& query_in, const at::Tensor& codes_k, const std::optional<at::Tensor>& codes_v,
@@ -490,6 +658,15 @@ TORCH_LIBRARY(fused_tq, m) {
         "int num_splits, Tensor(a!) workspace, Tensor(b!) out, Tensor(c!)? lse, Tensor? rotation) -> ()");
   m.def("v1_chunk_attention(Tensor query, Tensor kv_cache, Tensor block_row, int past_len, Tensor? centroids, "
         "int key_bits, int value_bits, float scale, int v_flags, int window, Tensor(a!) out, Tensor? rotation) -> ()");
+  m.def("v1_tree_attention(Tensor query, Tensor kv_cache, Tensor block_table, Tensor seq_lens, Tensor query_start_loc, "
+        "Tensor? tree_mask, Tensor? kv_start, Tensor? centroids, int key_bits, int value_bits, float scale, int v_flags, "
+        "int max_query_len, int num_splits, Tensor(a!) workspace, Tensor(b!) out, Tensor(c!)? lse, Tensor? rotation) -> ()");
+  m.def("step_tables(Tensor query_start_loc, Tensor past_lens, Tensor? depths, Tensor(a!) block_table, int block_size, "
+        "int num_tokens, Tensor(b!)? num_blocks, Tensor(c!)? free_blocks, Tensor(d!)? free_count) -> "
+        "(Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("tree_accept(Tensor tokens, Tensor parents, Tensor targets, Tensor query_start_loc, int max_nodes) -> "
+        "(Tensor, Tensor, Tensor)");
+  m.def("commit_slots(Tensor(a!)[] kv_caches, Tensor block_table, Tensor past_lens, Tensor path, Tensor counts) -> ()");
   m.def("lib_attention(Tensor query, Tensor codes_k, Tensor? codes_v, Tensor? norms_k, Tensor? norms_v, "
         "Tensor? block_table, Tensor lens, Tensor? new_key, Tensor? new_value, Tensor k_signs, Tensor v_signs, "
         "Tensor k_levels, Tensor v_levels, int bits_k, int bits_v, int max_len, float scale, int window, int sinks, "
@@ -512,6 +689,10 @@ TORCH_LIBRARY_IMPL(fused_tq, CUDA, m) {
   m.impl("v1_store", &v1_store);
   m.impl("v1_decode_attention", &v1_decode_attention);
   m.impl("v1_chunk_attention", &v1_chunk_attention);
+  m.impl("v1_tree_attention", &v1_tree_attention);
+  m.impl("step_tables", &step_tables);
+  m.impl("tree_accept", &tree_accept);
+  m.impl("commit_slots", &commit_slots);
   m.impl("lib_attention", &lib_attention);
   m.impl("rope", &rope);
   m.impl("append_slots", &append_slots);

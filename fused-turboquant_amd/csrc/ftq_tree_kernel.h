@@ -1,0 +1,421 @@
+// Attention of a tree of drafted tokens over the slot cache (speculative
+// decoding): sequence b has n_b query tokens, stored at its last n_b positions
+// c_b + j, and token i attends the context positions [start_i, c_b) and the
+// tokens j whose bit is set in its mask row (without masks, a chain: j <= i).
+//
+// The decode kernels give one query token a sequence a wave's 16 matrix
+// columns; n_b tokens through them would dequantise the cache n_b times.  Here a
+// workgroup (4 waves) takes 64 CT columns, a column being a (token, head of the
+// kv head's group) pair, dequantises each tile of TK positions once into LDS as
+// matrix-core operands, and every wave reads these for its 16 CT columns:
+//   S^T = K Q^T, softmax in the log2 domain with a lazily raised maximum,
+//   O^T = V^T P^T (v_mfma_f32_16x16x32_f16, float32 sums).
+// The context is split over workgroups where the columns alone do not fill the
+// GPU, and the parts meet in merge_splits_kernel.
+//
+// Operands in LDS, in the order in which lane (m, g) (m = lane & 15, g = lane >> 4)
+// reads its 16 bytes:
+//   K  [16-position tile][32-dim step s][part]: position m, dims 32 s + 8 g + j
+//   V  [32-position tile][block b][part]: dim NB m + b, positions 4 g + j and
+//      16 + 4 g + j (j < 4) -- the rows of the S^T accumulators, so that the weights
+//      go from the score registers into the product without a shuffle
+// and 4 floats a position: K factor, bias (0, or -inf without a page), V factor,
+// V minimum.
+#pragma once
+
+#include "ftq_attn_dev.h"
+#include "ftq_chunk_kernel.h"  // f16 pairs, the butterflies across lane rows
+#include "ftq_merge.h"
+#include "ftq_v1_dev.h"
+
+#include <type_traits>
+
+namespace ftq {
+
+struct TreeArgs {
+  const void* q;            // [tokens][hq][D]
+  int qt, tokens;
+  const uint8_t* cache;
+  int64_t nb, sblk, spos, shead;
+  int lbs;                  // log2 of the block size
+  const int32_t* bt;        // [B][max_blocks]
+  int max_blocks;
+  const int32_t *sl, *qsl;  // seq_lens [B], query_start_loc [B + 1]
+  const int32_t* ks;        // first context position of each token, or null
+  const uint64_t* mask;     // [tokens][words], or null (a chain)
+  int words;
+  int B, hq, hkv;
+  const float* cent;
+  int kb, vb, flags;
+  float qscale;             // of the (unnormalised) rotated query: scale log2 e, and the rotation's norm
+  int splits, nblk;         // grid: column blocks x splits x B x hkv
+  float *wo, *wl;           // partial outputs / log-sum-exps, or
+  void* out;                // the output itself (wo == null)
+  int ot, unrot;            // its type; whether V is taken back by H
+  float oscale;
+  float* lse;               // with a direct output, or null
+  const float* rot;         // matrix of the rotation strategy, or null
+};
+
+constexpr int TREE_RAW = 16;  // key_bits of raw fp16 slots
+
+template <int D> struct TreeGeo {
+  static constexpr int CT = D == 256 ? 1 : 2;     // 16-column tiles per wave
+  static constexpr int TK = D == 64 ? 64 : 32;    // positions of a tile
+  static constexpr int NS = D / 32, NB = D / 16, NT = TK / 16, NP = TK / 32;
+};
+
+// The sequence, kv head and columns of a workgroup.  Workgroups are dealt to
+// the 8 XCDs in turn; with the kv head fastest, those that read the same slots
+// (the column blocks and splits of one kv head) share an XCD's L2 when there
+// are 8 heads or a multiple.
+struct TreeUnit {
+  int b, kvh, split, blk;
+  int q0, n, ctx, len;      // first query token, query tokens, context positions, all positions
+  __device__ __forceinline__ explicit TreeUnit(const TreeArgs& a) {
+    int id = (int)blockIdx.x;
+    kvh = id % a.hkv;
+    id /= a.hkv;
+    b = id % a.B;
+    id /= a.B;
+    split = id % a.splits;
+    blk = id / a.splits;
+    q0 = min(max(a.qsl[b], 0), a.tokens);
+    n = max(min(a.qsl[b + 1], a.tokens) - q0, 0);
+    len = max(a.sl[b], n);
+    ctx = len - n;
+  }
+};
+
+// Bits of row t's mask (null: tokens up to row r of its own) for the 32 positions from
+// pos0 on, the context's from `start` on among them.
+__device__ __forceinline__ uint32_t tree_visible(const TreeArgs& a, const TreeUnit& u, int t, int r, int start, int pos0) {
+  auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; };  // bits 0 .. k - 1
+  const int rel = pos0 - u.ctx;  // tree token of bit 0
+  uint32_t v = below(-rel) & ~below(start - pos0);
+  uint32_t w = 0;
+  if (rel > -32 && rel < u.n) {
+    if (a.mask == nullptr) {
+      w = below(r + 1 - rel) & ~below(-rel);
+    } else {
+      const uint64_t* row = a.mask + (int64_t)t * a.words;
+      if (rel < 0) {
+        w = (uint32_t)(row[0] << -rel);
+      } else {
+        const int i = rel >> 6, o = rel & 63;
+        if (i < a.words) w = (uint32_t)(row[i] >> o);
+        if (o > 32 && i + 1 < a.words) w |= (uint32_t)(row[i + 1] << (64 - o));
+      }
+      w &= below(u.n - rel);
+    }
+  }
+  return v | w;
+}
+
+// One wave's columns.  KHL: K as f16 hi + lo; NHP: f16 parts of the weights (the
+// query always has two); VHL: V as hi + lo (Lloyd-Max V).
+template <int D, int CT, bool KHL, int NHP, bool VHL>
+struct TreeWave {
+  using C = TreeGeo<D>;
+  static constexpr int TK = C::TK, NS = C::NS, NB = C::NB, NT = C::NT, NP = C::NP;
+  static constexpr int KP = KHL ? 2 : 1, VP = VHL ? 2 : 1;
+  static constexpr int KU = NT * NS * KP * 64, VU = NP * NB * VP * 64;  // 16-byte units of a tile
+  static constexpr float TAU = 4.f;        // weights stay below 2^TAU
+  static constexpr float MINF = -3.0e38f;  // running maximum of a column with no position yet
+
+  half8 qh[CT][NS], ql[CT][NS];
+  float qs[CT];                            // of the scores: 1, or what a query beyond f16's range was divided by
+  bool qlarge;                             // some qs is not 1 (wave-uniform)
+  float m_run[CT], l_run[CT], z_run[CT];
+  floatx4 acc[CT][NB];
+  int row[CT], tok[CT], start[CT];         // query row in the sequence, its token, its first context position
+  bool live[CT];
+
+  __device__ __forceinline__ void columns(const TreeArgs& a, const TreeUnit& u, int c0, int lane) {
+    const int G = a.hq / a.hkv, n = lane & 15;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int col = c0 + 16 * ct + n;
+      live[ct] = col < u.n * G;
+      row[ct] = live[ct] ? col / G : 0;
+      tok[ct] = u.q0 + row[ct];
+      start[ct] = live[ct] && a.ks != nullptr ? max(a.ks[tok[ct]], 0) : 0;
+      m_run[ct] = MINF;
+      l_run[ct] = z_run[ct] = 0.f;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) acc[ct][b] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  // The columns' queries, rotated and scaled, as f16 hi + lo.  One query per 16
+  // lanes, four at a time, through 16 rows of LDS of the wave's own.
+  __device__ __forceinline__ void queries(const TreeArgs& a, const TreeUnit& u, int c0, int lane, float (*rows)[D + 4]) {
+    constexpr int E = D / 16;
+    const int G = a.hq / a.hkv, l16 = lane & 15, g = lane >> 4, n = lane & 15;
+    qlarge = false;
+#pragma unroll 1
+    for (int ct = 0; ct < CT; ++ct) {
+      float inv = 1.f;
+#pragma unroll 1
+      for (int k = 0; k < 4; ++k) {
+        const int col = c0 + 16 * ct + 4 * k + g;
+        const bool on = col < u.n * G;
+        const int r = on ? col / G : 0, h = u.kvh * G + (on ? col - r * G : 0);
+        float y[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) y[i] = 0.f;
+        if (on) {
+          const int64_t off = ((int64_t)(u.q0 + r) * a.hq + h) * D + l16 * E;
+          if (a.qt == F32) load_elems<F32, E>(a.q, off, y);
+          else if (a.qt == F16) load_elems<F16, E>(a.q, off, y);
+          else load_elems<BF16, E>(a.q, off, y);
+        }
+        if (a.kb != TREE_RAW) {
+          if (a.rot != nullptr) rot_matrix_lanes<D, E>(y, a.rot, rows[4 * k + g], l16);
+          else fwht_lanes<E, 16>(y, l16);
+        }
+        float mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          y[i] *= a.qscale;
+          mx = fmaxf(mx, fabsf(y[i]));
+        }
+        mx = fmaxf(mx, lane_xor<1>(mx));
+        mx = fmaxf(mx, lane_xor<2>(mx));
+        mx = fmaxf(mx, lane_xor<4>(mx));
+        mx = fmaxf(mx, lane_xor<8>(mx));
+        // A query that f16 cannot hold is scaled to [2^13, 2^14).  Small ones need
+        // no scale: what their low parts lose below f16's range is 2^-25 of a
+        // score, an absolute error.
+        const int e = (int)((__float_as_uint(mx) >> 23) & 255u);
+        const int ue = e >= 127 + 14 && e < 255 ? 140 + 127 - e : 127;
+        const float up = __uint_as_float((uint32_t)ue << 23);
+        const float down = __uint_as_float((uint32_t)(254 - ue) << 23);
+        const float got = __shfl(down, (n & 3) << 4);  // of column 4 k + (n & 3)
+        if ((n >> 2) == k) inv = got;
+#pragma unroll
+        for (int i = 0; i < E; ++i) rows[4 * k + g][l16 * E + i] = y[i] * up;
+      }
+      __asm__ volatile("" ::: "memory");  // a wave's LDS accesses run in order
+      half8 hi[NS], lo[NS];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = rows[n][32 * s + 8 * g + 2 * j], y = rows[n][32 * s + 8 * g + 2 * j + 1];
+          h[j] = pk_f16(x, y);
+          l[j] = pk_f16(f16_rest(x, h[j], 0), f16_rest(y, h[j], 1));
+        }
+        hi[s] = __builtin_bit_cast(half8, u32x4{h[0], h[1], h[2], h[3]});
+        lo[s] = __builtin_bit_cast(half8, u32x4{l[0], l[1], l[2], l[3]});
+      }
+      __asm__ volatile("" ::: "memory");
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+        if (c == ct) {  // (register arrays need constant indexes)
+          qs[c] = inv;
+#pragma unroll
+          for (int s = 0; s < NS; ++s) {
+            qh[c][s] = hi[s];
+            ql[c][s] = lo[s];
+          }
+        }
+      qlarge = qlarge || __builtin_amdgcn_ballot_w64(inv != 1.f) != 0;
+    }
+  }
+
+  // One tile: kb, vb its operands, tb its factors.  vis: bits of the positions
+  // that each column attends (edge tiles only).  next(): called once this tile's
+  // operands are in registers.
+  template <bool EDGE, typename F>
+  __device__ __forceinline__ void tile(const u32x4* kb, const u32x4* vb, const float (*tb)[TK], const uint32_t (&vis)[CT][NP],
+                                       int lane, F next) {
+    const int g = lane >> 4;
+    floatx4 s[NT][CT];
+#pragma unroll
+    for (int k = 0; k < NT; ++k)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) s[k][ct] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < NS; ++d) {
+      half8 xh[NT], xl[NT];
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        xh[k] = __builtin_bit_cast(half8, kb[((k * NS + d) * KP) * 64 + lane]);
+        if constexpr (KHL) xl[k] = __builtin_bit_cast(half8, kb[((k * NS + d) * KP + 1) * 64 + lane]);
+      }
+      // the low products first: what they add is not lost beside the high ones' sum
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[k], ql[ct][d], s[k][ct], 0, 0, 0);
+      if constexpr (KHL) {
+#pragma unroll
+        for (int k = 0; k < NT; ++k)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl[k], qh[ct][d], s[k][ct], 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[k], qh[ct][d], s[k][ct], 0, 0, 0);
+    }
+    half8 xv[NP * NB];
+#pragma unroll
+    for (int i = 0; i < NP * NB; ++i) xv[i] = __builtin_bit_cast(half8, vb[i * VP * 64 + lane]);
+    float tf[NT][4][4];  // the factors of this lane's positions 16 k + 4 g + i
+#pragma unroll
+    for (int k = 0; k < NT; ++k)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        const float4 x = *reinterpret_cast<const float4*>(&tb[f][16 * k + 4 * g]);
+        tf[k][f][0] = x.x; tf[k][f][1] = x.y; tf[k][f][2] = x.z; tf[k][f][3] = x.w;
+      }
+    next();
+    if (qlarge) {
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) s[k][ct] *= qs[ct];
+    }
+#pragma unroll
+    for (int k = 0; k < NT; ++k)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[k][ct][i] = __builtin_fmaf(s[k][ct][i], tf[k][0][i], tf[k][1][i]);
+    if constexpr (EDGE) {
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (((vis[ct][k >> 1] >> (16 * (k & 1) + 4 * g + i)) & 1u) == 0) s[k][ct][i] = -INFINITY;
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float tm = s[0][ct][0];
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tm = fmaxf(tm, s[k][ct][i]);
+      tm = warp_max_q(tm);
+      if (__builtin_amdgcn_ballot_w64(tm > m_run[ct] + TAU) != 0) {  // wave-uniform, rare
+        const float mn = fmaxf(m_run[ct], tm);
+        const float al = __builtin_amdgcn_exp2f(m_run[ct] - mn);
+        m_run[ct] = mn;
+        l_run[ct] *= al;
+        z_run[ct] *= al;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[ct][b] *= al;
+      }
+    }
+    // weights: p; p x V minimum kept aside; p x V factor as f16 parts.  A tile's
+    // sums are formed first, so that many small weights beside a large one count.
+    u32x4 ph[NP][CT], pl[NP][CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float lt = 0.f, zt = 0.f;
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool hid = EDGE && s[k][ct][i] == -INFINITY;  // its factors may be infinite or NaN
+          const float e = __builtin_amdgcn_exp2f(s[k][ct][i] - m_run[ct]);
+          lt += e;
+          zt = __builtin_fmaf(e, hid ? 0.f : tf[k][3][i], zt);
+          w[i] = e * (hid ? 0.f : tf[k][2][i]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t hi = pk_f16(w[2 * h], w[2 * h + 1]);
+          ph[k >> 1][ct][2 * (k & 1) + h] = hi;
+          if constexpr (NHP == 2) pl[k >> 1][ct][2 * (k & 1) + h] = pk_f16(f16_rest(w[2 * h], hi, 0), f16_rest(w[2 * h + 1], hi, 1));
+        }
+      }
+      l_run[ct] += lt;
+      z_run[ct] += zt;
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        if constexpr (VHL) {
+          const half8 x = __builtin_bit_cast(half8, vb[((p * NB + b) * VP + 1) * 64 + lane]);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+            acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(half8, ph[p][ct]), acc[ct][b], 0, 0, 0);
+        }
+        if constexpr (NHP == 2) {
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+            acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xv[p * NB + b], __builtin_bit_cast(half8, pl[p][ct]), acc[ct][b], 0, 0, 0);
+        }
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+          acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xv[p * NB + b], __builtin_bit_cast(half8, ph[p][ct]), acc[ct][b], 0, 0, 0);
+      }
+  }
+
+  // Lane (n, g) holds dims NB (4 g + i) + b of column n.  vscale undoes the common
+  // power of two of the weights' factors.
+  __device__ __forceinline__ void finish(const TreeArgs& a, const TreeUnit& u, int c0, int lane, float vscale) {
+    const int n = lane & 15, g = lane >> 4, G = a.hq / a.hkv;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const float L = warp_sum_q(l_run[ct]), Z = warp_sum_q(z_run[ct]);
+      const bool none = L == 0.f;  // no position; a NaN score makes L, and the output, NaN
+      const float inv = none ? 0.f : 1.f / L;
+      float y[4][NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i][b] = none ? 0.f : __builtin_fmaf(acc[ct][b][i], vscale, Z) * inv;
+      const int64_t at = (int64_t)tok[ct] * a.hq + u.kvh * G + (c0 + 16 * ct + n - row[ct] * G);
+      if (a.wo != nullptr) {
+        if (live[ct]) {
+          const int64_t r = at * a.splits + u.split;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) store_elems<F32, NB>(a.wo, r * D + NB * (4 * g + i), y[i]);
+          if (g == 0) a.wl[r] = none ? -INFINITY : m_run[ct] + __builtin_log2f(L);
+        }
+        continue;
+      }
+      if (a.unrot) {  // H o: the low dim bits in registers, the top two across the lane rows
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int st = 1; st < NB; st <<= 1)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              if ((b & st) == 0) {
+                const float v0 = y[i][b], v1 = y[i][b + st];
+                y[i][b] = v0 + v1;
+                y[i][b + st] = v0 - v1;
+              }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const float u0 = y[0][b] + y[1][b], u1 = y[0][b] - y[1][b], u2 = y[2][b] + y[3][b], u3 = y[2][b] - y[3][b];
+          y[0][b] = u0 + u2; y[1][b] = u1 + u3; y[2][b] = u0 - u2; y[3][b] = u1 - u3;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i][b] = fwht_pair32(fwht_pair16(y[i][b], g & 1), g & 2) * a.oscale;
+        }
+      }
+      if (live[ct]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t off = at * D + NB * (4 * g + i);
+          if (a.ot == F32) store_elems<F32, NB>(a.out, off, y[i]);
+          else if (a.ot == F16) store_elems<F16, NB>(a.out, off, y[i]);
+          else store_elems<BF16, NB>(a.out, off, y[i]);
+        }
+        if (a.lse != nullptr && g == 0) a.lse[at] = none ? -INFINITY : (m_run[ct] + __builtin_log2f(L)) * 0.69314718055994531f;
+      }
+    }
+  }
+};
+
+}  // namespace ftq

@@ -57,9 +57,21 @@ def _register_fakes() -> None:
     def _append_slots(lens, n, capacity):
         return lens.new_empty((lens.numel() * n,), dtype=torch.int64)
 
+    @torch.library.register_fake(lib + "step_tables")
+    def _step_tables(query_start_loc, past_lens, depths, block_table, block_size, num_tokens, num_blocks, free_blocks, free_count):
+        new = past_lens.new_empty
+        return (new((num_tokens,), dtype=torch.int64), new((num_tokens,), dtype=torch.int64), new((num_tokens,)),
+                new(past_lens.shape), new((1,)))
+
+    @torch.library.register_fake(lib + "tree_accept")
+    def _tree_accept(tokens, parents, targets, query_start_loc, max_nodes):
+        B = query_start_loc.shape[0] - 1
+        return (parents.new_empty((B, max_nodes)), parents.new_empty((B,)), tokens.new_empty((B, max_nodes)))
+
     # operators that only write their (a!) arguments
     for name in ("paged_store", "paged_decode_attention", "v1_store", "v1_decode_attention",
-                 "v1_chunk_attention", "lib_attention", "raw_store", "raw_decode_attention"):
+                 "v1_chunk_attention", "v1_tree_attention", "lib_attention", "raw_store", "raw_decode_attention",
+                 "commit_slots"):
         torch.library.register_fake(lib + name)(lambda *args, **kwargs: None)
 
 

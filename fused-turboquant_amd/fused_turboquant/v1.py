@@ -71,6 +71,8 @@ def _bind():
     L.ftq_v1_default_splits.argtypes = [ctypes.c_int] * 3
     L.ftq_v1_choose_splits.restype = ctypes.c_int
     L.ftq_v1_choose_splits.argtypes = [ctypes.c_int] * 8
+    L.ftq_v1_tree_choose_splits.restype = ctypes.c_int
+    L.ftq_v1_tree_choose_splits.argtypes = [ctypes.c_int] * 9
     L._v1_bound = True
     return L
 
@@ -481,6 +483,105 @@ def v1_chunk_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_row: t
     return out
 
 
+def default_tree_splits(batch: int, max_query_len: int, num_q_heads: int, num_kv_heads: int, head_dim: int, key_bits: int,
+                        value_bits: int, max_seq_len: int, v_flags: int = 0) -> int:
+    """Split-K factor of ``v1_tree_attention`` that fills the GPU (``ftq_v1_tree_choose_splits``)."""
+    return int(_bind().ftq_v1_tree_choose_splits(batch, max_query_len, num_q_heads, num_kv_heads, head_dim, key_bits,
+                                                 value_bits, v_flags, max_seq_len))
+
+
+def v1_tree_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                      query_start_loc: torch.Tensor, centroids: torch.Tensor | None, key_bits: int, value_bits: int,
+                      tree_mask: torch.Tensor | None = None, scale: float | None = None, v_rotate: bool = False,
+                      v_lloyd_max: bool = False, kv_start: torch.Tensor | None = None, num_splits: int | None = None,
+                      max_query_len: int | None = None, max_seq_len: int | None = None,
+                      out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                      lse: torch.Tensor | None = None, rotation: torch.Tensor | None = None,
+                      sorted_centroids: bool = False, key_fp8: bool = False) -> torch.Tensor:
+    """Attention of several query tokens per sequence, the nodes of a drafted
+    tree or a chain: query [T, Hq, d] -> [T, Hq, d] (query dtype unless ``out``
+    is given).
+
+    Sequence b has the flat tokens ``query_start_loc[b] ..
+    query_start_loc[b + 1]`` (int32 [B + 1], from 0, ascending), stored at its
+    last n positions: ``seq_lens[b]`` (int32) counts them.  Token i attends the
+    context positions [kv_start, seq_lens[b] - n) and the tokens j of its
+    sequence whose bit j is set in its row of ``tree_mask`` (int64 [T, words],
+    bit j in word j // 64; a node's ancestors and itself); without a mask the
+    tokens up to its own.  ``kv_start`` (int32 [T]) is per token, None = 0.  A
+    token that attends nothing gets 0 (``lse`` -inf).  Rows behind
+    ``query_start_loc[B]`` are left as they were.
+
+    ``key_bits = value_bits = RAW_BITS`` reads raw fp16 slots (``centroids``
+    None); every other format of ``v1_decode_attention`` is taken.
+    ``max_query_len`` and ``max_seq_len`` (host numbers, default T and the
+    table's width) only size the launch and ``num_splits``; ``workspace``
+    (uint8, ``workspace_bytes(T, ...)``) may be preallocated for graph capture.
+    ``lse`` (float32 [T, Hq]) as in ``v1_decode_attention``.
+    """
+    T, hq, d = query.shape
+    raw = key_bits == RAW_BITS
+    if kv_cache.dim() != 4:
+        raise ValueError("kv_cache must be uint8 [num_blocks, block_size, num_kv_heads, slot]")
+    nb, bs, hkv, slot = kv_cache.shape
+    if raw:
+        if value_bits != RAW_BITS or v_rotate or v_lloyd_max or key_fp8 or rotation is not None:
+            raise ValueError("raw slots: key_bits = value_bits = RAW_BITS, no rotation, Lloyd-Max or fp8 keys")
+        if slot < 4 * d:
+            raise ValueError("kv_cache slot is smaller than 4 * head_dim bytes")
+        centroids = None
+    else:
+        _check_bits(d, key_bits, value_bits, key_fp8)
+        if slot < slot_bytes(d, key_bits, value_bits, key_fp8):
+            raise ValueError("kv_cache slot is smaller than the slot bytes for these bits")
+        if key_fp8:
+            centroids = None
+        elif centroids is None or centroids.numel() != 1 << key_bits:
+            raise ValueError("centroids must have 2^key_bits entries")
+    if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 or query_start_loc.dtype != torch.int32:
+        raise ValueError("block_table, seq_lens and query_start_loc must be int32")
+    B = seq_lens.numel()
+    if block_table.dim() != 2 or block_table.shape[0] != B or query_start_loc.numel() != B + 1:
+        raise ValueError("block_table must be [B, max_blocks], seq_lens [B] and query_start_loc [B + 1]")
+    if tree_mask is not None and (tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != T or
+                                  tree_mask.shape[1] < 1):
+        raise ValueError("tree_mask must be int64 [T, words]")
+    if kv_start is not None and (kv_start.dtype != torch.int32 or kv_start.numel() != T):
+        raise ValueError("kv_start must be int32 [T]")
+    if lse is not None and (lse.dtype != torch.float32 or lse.numel() != T * hq or not lse.is_contiguous()):
+        raise ValueError("lse must be a contiguous float32 tensor of T * num_q_heads entries")
+    if max_query_len is not None and (max_query_len < 0 or (max_query_len == 0 and T > 0)):
+        raise ValueError("max_query_len must be positive")
+    dev = _lib.require_device(query, kv_cache, block_table, seq_lens, query_start_loc, centroids, tree_mask, kv_start, lse)
+    q = query.contiguous()
+    if q.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        q = q.float()
+    if out is None:
+        out = torch.empty(T, hq, d, dtype=q.dtype, device=dev)
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    mql = min(max_query_len, T) if max_query_len is not None else T
+    flags = 0 if raw else _v_flags(v_rotate, v_lloyd_max, key_fp8)
+    if num_splits is None:
+        msl = max_seq_len if max_seq_len is not None else block_table.shape[1] * bs
+        num_splits = default_tree_splits(B, mql, hq, hkv, d, key_bits, value_bits, msl, flags)
+    need = workspace_bytes(T, hq, d, num_splits)
+    if workspace is None or workspace.numel() < need:
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+    _strides(kv_cache)
+    if centroids is not None:
+        centroids = centroids.to(torch.float32)
+        if not sorted_centroids:
+            centroids = torch.sort(centroids).values
+        centroids = centroids.contiguous()
+    rot = _rotation_arg(rotation, d, dev) if rotation is not None else None
+    _ops.ops().v1_tree_attention(q, kv_cache, block_table.contiguous(), seq_lens.contiguous(), query_start_loc.contiguous(),
+                                 tree_mask.contiguous() if tree_mask is not None else None,
+                                 kv_start.contiguous() if kv_start is not None else None, centroids, key_bits, value_bits,
+                                 float(scale), flags, mql, int(num_splits), workspace, out, lse, rot)
+    return out
+
+
 class TurboQuantV1Layer:
     """Per-layer state of the v1 backend for ``kind=rht``: sorted centroids and
     midpoints (reference ``rotation/matrix.py:34-42``), bit widths and the
@@ -544,3 +645,9 @@ class TurboQuantV1Layer:
                                    v_lloyd_max=self.v_lloyd_max, rotation=self.rotation,
                                    sorted_centroids=True, key_fp8=self.key_fp8,
                                    **{"operands": self.operands, **kw})
+
+    def tree(self, query, kv_cache, block_table, seq_lens, query_start_loc, tree_mask=None, **kw) -> torch.Tensor:
+        return v1_tree_attention(query, kv_cache, block_table, seq_lens, query_start_loc, self.centroids, self.key_bits,
+                                 self.value_bits, tree_mask=tree_mask, v_rotate=self.v_rotate,
+                                 v_lloyd_max=self.v_lloyd_max, rotation=self.rotation, sorted_centroids=True,
+                                 key_fp8=self.key_fp8, **kw)

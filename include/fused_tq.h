@@ -409,6 +409,87 @@ int ftq_v1_chunk_attention(const void* query, int q_dtype, const uint8_t* kv_cac
                            void* out, int out_dtype, const float* rotation, void* stream);
 
 /*
+ * Attention of several query tokens per sequence over the slot cache: the
+ * nodes of a drafted tree (or a chain) of speculative decoding, all of them
+ * already stored.  Sequence b has the flat tokens query_start_loc[b] ..
+ * query_start_loc[b + 1] (int32 [batch + 1], from 0, ascending, within
+ * num_tokens), the last of its seq_lens[b] positions; token i attends the
+ * context positions [kv_start[token], seq_lens[b] - n) (kv_start [num_tokens],
+ * NULL = 0) and the tokens j whose bit is set in its row of tree_mask
+ * ([num_tokens][mask_words], bit j in word j / 64; NULL: j <= i).
+ *   query, out [num_tokens, num_q_heads, d]; rows behind the last sequence are
+ *   not written; a token that attends nothing gives 0 (lse -inf)
+ *   key_bits, value_bits, v_flags: as ftq_v1_decode_attention (bits 0, 1 and
+ *   2), or both 16 for raw fp16 slots (no flags, no rotation, no centroids)
+ *   max_query_len: the longest sequence's tokens; sizes the grid only
+ *   workspace: ftq_v1_workspace_bytes(num_tokens, num_q_heads, d, num_splits)
+ * One launch with one split (unless a caller's matrix un-rotates the output),
+ * else two.  No counterpart in the reference, which decodes one token a
+ * sequence.
+ */
+int ftq_v1_tree_attention(const void* query, int q_dtype, int64_t num_tokens, const uint8_t* kv_cache,
+                          int64_t num_blocks, int block_size, int64_t stride_block, int64_t stride_pos,
+                          int64_t stride_head, const int32_t* block_table, int max_blocks_per_seq,
+                          const int32_t* seq_lens, const int32_t* query_start_loc, const uint64_t* tree_mask,
+                          int mask_words, const int32_t* kv_start, int batch, int max_query_len,
+                          int num_q_heads, int num_kv_heads, int d, const float* centroids, int key_bits,
+                          int value_bits, float scale, int v_flags, int num_splits, void* workspace,
+                          int64_t workspace_bytes, void* out, int out_dtype, float* lse_out,
+                          const float* rotation, void* stream);
+/* Split-K factor that fills the GPU for such a call (host-side heuristic). */
+int ftq_v1_tree_choose_splits(int batch, int max_query_len, int num_q_heads, int num_kv_heads, int d,
+                              int key_bits, int value_bits, int v_flags, int max_seq_len);
+
+/*
+ * Slots, positions and lengths of a step's tokens from the requests' lengths:
+ * request b (of batch <= 4096) has the tokens query_start_loc[b] ..
+ * query_start_loc[b + 1] of num_tokens, stored from position past_lens[b] on.
+ *   slot_mapping[t] = table[b][pos / block_size] * block_size + pos % block_size,
+ *   -1 for padding (tokens behind the last request) and tokens without a page;
+ *   positions[t] = past_lens[b] + (depths ? depths[t] : index in the request),
+ *   token_request[t] = b (-1), seq_lens[b] = past_lens[b] + its tokens
+ * table_stride: int32 from one row of block_table to the next.
+ * num_blocks_held [batch], free_blocks [pool_size] and free_count [1] (all or
+ * none NULL): the tables are brought to ceil(seq_len / block_size) pages first.
+ * Pages released by shorter requests are appended to the free list (its first
+ * free_count entries) in the order of requests and pages, then new ones are
+ * taken from its end in that order; missing[0] counts the pages that it, or
+ * max_blocks, lacked.  One launch up to 4096 tokens, else two with a free list.
+ * No counterpart in the reference (vLLM's host-side metadata builder).
+ */
+int ftq_step_tables(const int32_t* query_start_loc, const int32_t* past_lens, const int32_t* depths, int batch,
+                    int64_t num_tokens, int32_t* block_table, int64_t table_stride, int max_blocks, int block_size,
+                    int32_t* num_blocks_held, int32_t* free_blocks, int32_t* free_count, int pool_size,
+                    int64_t* slot_mapping, int64_t* positions, int32_t* token_request, int32_t* seq_lens,
+                    int32_t* missing, void* stream);
+
+/*
+ * The accepted path of each drafted tree: nodes query_start_loc[b] ..
+ * query_start_loc[b + 1] of num_tokens, the root first, with their tokens,
+ * parents (index in the tree, before the node's own) and the target model's
+ * token after each.  From the root to the lowest child whose token is the
+ * current node's target, until there is none.
+ *   path, accepted [batch][max_nodes]: the nodes and their targets, then -1;
+ *   counts [batch].  max_nodes in [1, 2048]; nodes past it are not read.
+ */
+int ftq_tree_accept(const int64_t* tokens, const int32_t* parents, const int64_t* targets,
+                    const int32_t* query_start_loc, int batch, int64_t num_tokens, int max_nodes, int32_t* path,
+                    int32_t* counts, int64_t* accepted, void* stream);
+
+/*
+ * Move the slots of accepted paths together, in place: in each of num_caches
+ * caches (HOST array of device pointers, one shape and layout, none twice)
+ * position past_lens[b] + path[b][j] goes to past_lens[b] + j, j < counts[b]
+ * (path [batch][max_nodes], ascending; an entry that does not ascend ends it).
+ * Positions without a page are skipped.  One launch per 64 caches.
+ */
+int ftq_commit_slots(uint8_t* const* kv_caches, int num_caches, int64_t num_blocks, int block_size,
+                     int64_t stride_block, int64_t stride_pos, int64_t stride_head, int num_kv_heads,
+                     int slot_bytes, const int32_t* block_table, int64_t table_stride, int max_blocks,
+                     const int32_t* past_lens, const int32_t* path, const int32_t* counts, int max_nodes,
+                     int batch, void* stream);
+
+/*
  * Attention over a library-format cache (pages of ftq_paged_store, or flat
  * codes and norms per sequence) for the calls that
  * ftq_paged_decode_attention does not take; d = 64, 128 or 256:

@@ -11,6 +11,9 @@ namespace ftq {
 
 float fwht_scale(int d);
 bool v1_widths_ok(int kb, int vb, int flags);
+hipError_t tree_fast_64(const TreeArgs& a, unsigned grid, hipStream_t st);
+hipError_t tree_fast_128(const TreeArgs& a, unsigned grid, hipStream_t st);
+hipError_t tree_fast_256(const TreeArgs& a, unsigned grid, hipStream_t st);
 
 namespace {
 
@@ -54,10 +57,9 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
   using W = TreeWave<D, CT, true, 2, LM>;
   constexpr int LPT = 256 / TK, DPL = D / LPT;  // lanes of a position, their dims
   extern __shared__ __attribute__((aligned(16))) uint32_t pool[];  // slots [TK][pitch]; before: query rows; both: operands behind
-  __shared__ __attribute__((aligned(16))) float tb[4][TK];
+  __shared__ __attribute__((aligned(16))) float tb[3][TK];
   __shared__ uint32_t tabk[256], tabv[16];  // f16 hi | lo << 16 of the scaled table
   __shared__ float tabn[256];
-  __shared__ int ok[TK];
   __shared__ float vex[TK];                 // 2^e of the position's V operand
   __shared__ float table_scale_inv;
   __shared__ int red[4][2];
@@ -99,22 +101,9 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
     w.columns(a, u, c0, lane);
     __syncthreads();  // the pool is free (and the tables written)
     w.queries(a, u, c0, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
-    int first = u.len, last = 0;  // first positions of the workgroup's columns
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
-      if (w.live[ct]) {
-        first = min(first, w.start[ct]);
-        last = max(last, w.start[ct]);
-      }
-    first = (int)wave_min_u32((uint32_t)first);
-    last = (int)~wave_min_u32(~(uint32_t)last);
-    if (lane == 0) {
-      red[wave][0] = first;
-      red[wave][1] = last;
-    }
-    __syncthreads();
-    first = min(min(min(red[0][0], red[1][0]), min(red[2][0], red[3][0])), u.ctx);  // the tree's own positions always
-    last = max(max(red[0][1], red[1][1]), max(red[2][1], red[3][1]));
+    int first, last;
+    w.starts(u.len, lane, wave, red, first, last);
+    first = min(first, u.ctx);  // the tree's own positions always
     const int held = (int)min((int64_t)u.len, (int64_t)a.max_blocks << a.lbs);  // positions that can have a page
     const int t0 = first / TK, t1 = max((held + TK - 1) / TK, t0);
     const int per = (t1 - t0 + a.splits - 1) / a.splits;
@@ -134,10 +123,7 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
           rows[p * pitch + c] = x;
           if (raw && c >= D / 2 && ((x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u)) beyond = 1.f;
         }
-        if (sub == 0) {
-          ok[p] = on;
-          rows[p * pitch + nd] = 0;
-        }
+        if (sub == 0) rows[p * pitch + nd] = 0;
       }
       __syncthreads();
       {  // factors
@@ -177,18 +163,16 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
             vs = sc * __uint_as_float((uint32_t)(127 - e) << 23) * tree_lift(false);
             if (!LM) vm = __builtin_fmaf(mid, sc, f16_bits_to_f32(row_bits(row, 8 * (geo.kps + geo.vdb) + 16, 16)));
           }
-          const bool on = ok[p] != 0;
-          tb[0][p] = on ? fk : 0.f;
-          tb[1][p] = on ? 0.f : -INFINITY;
-          tb[2][p] = on ? vs : 0.f;
-          tb[3][p] = on ? vm : 0.f;
+          tb[0][p] = fk;
+          tb[1][p] = vs;
+          tb[2][p] = vm;
           vex[p] = ve;
         }
       }
       __syncthreads();
       for (int i = tid; i < NT * NS * 64; i += 256) {
         const int l = i & 63, ts = i >> 6, m = l & 15, g = l >> 4;
-        const int d0 = (ts % NS) * 32 + 8 * g;
+        const int d0 = (ts % NS) * 32 + 8 * g, at = (ts / NS) * 2 * NS * 64 + C::kunit(ts % NS, m, g);
         const uint32_t* row = rows + ((ts / NS) * 16 + m) * pitch;
         uint32_t h[4], lo[4];
 #pragma unroll
@@ -202,8 +186,8 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
             lo[j] = (x >> 16) | (y & 0xffff0000u);
           }
         }
-        kf[ts * 2 * 64 + l] = u32x4{h[0], h[1], h[2], h[3]};
-        kf[(ts * 2 + 1) * 64 + l] = u32x4{lo[0], lo[1], lo[2], lo[3]};
+        kf[at] = u32x4{h[0], h[1], h[2], h[3]};
+        kf[at + NS * 64] = u32x4{lo[0], lo[1], lo[2], lo[3]};
       }
       for (int i = tid; i < NP * NB * 64; i += 256) {
         const int l = i & 63, pb = i >> 6, m = l & 15, g = l >> 4, d = NB * m + pb % NB;
@@ -213,7 +197,7 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
           float x[2], y[2];  // hi and lo of two positions
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const int p = (pb / NB) * 32 + (j >> 1) * 16 + 4 * g + 2 * (j & 1) + k;
+            const int p = (pb / NB) * 32 + ((j >> 1) ^ (C::vx(pb % NB) ? 1 : 0)) * 16 + 4 * g + 2 * (j & 1) + k;
             const uint32_t* row = rows + p * pitch;
             y[k] = 0.f;
             if (raw) {
@@ -229,22 +213,13 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
           h[j] = pk_f16(x[0], x[1]);
           if constexpr (LM) lo[j] = pk_f16(y[0], y[1]);
         }
-        vf[pb * W::VP * 64 + l] = u32x4{h[0], h[1], h[2], h[3]};
-        if constexpr (LM) vf[(pb * 2 + 1) * 64 + l] = u32x4{lo[0], lo[1], lo[2], lo[3]};
+        const int at = ((pb / NB) * W::VP * NB + pb % NB) * 64 + l;
+        vf[at] = u32x4{h[0], h[1], h[2], h[3]};
+        if constexpr (LM) vf[at + NB * 64] = u32x4{lo[0], lo[1], lo[2], lo[3]};
       }
       __syncthreads();
-      uint32_t vis[CT][NP];
-      const bool edge = pos0 < last || pos0 + TK > u.ctx;
-      if (edge) {
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-          for (int p = 0; p < NP; ++p)
-            vis[ct][p] = w.live[ct] ? tree_visible(a, u, w.tok[ct], w.row[ct], w.start[ct], pos0 + 32 * p) : 0u;
-        w.template tile<true>(kf, vf, tb, vis, lane, [] {});
-      } else {
-        w.template tile<false>(kf, vf, tb, vis, lane, [] {});
-      }
+      const uint32_t on = tree_held<TK>(a, u, pos0);  // bit k: positions 16 k .. of the tile have a page
+      w.tile(a, u, kf, vf, tb, pos0, pos0 < last || pos0 + TK > u.ctx || on != (1u << NT) - 1u, on, lane, [] {});
       __syncthreads();  // before the next tile's rows
     }
     w.finish(a, u, c0, lane, 1.f / tree_lift(raw));
@@ -279,11 +254,20 @@ hipError_t tree_merge(const TreeArgs& a, int64_t tokens, bool vrot, hipStream_t 
 #undef FTQ_TREE_MERGE
 }
 
+// The formats of ftq_tree_fast.h: 16-bit outputs, 2-4 bit codes or raw slots that
+// 16-byte loads reach, and positions of a tile within 32-bit offsets.
+bool tree_fast_takes(const TreeArgs& a) {
+  if (a.ot == F32 || a.spos > (1 << 26)) return false;
+  if (a.kb == TREE_RAW) return (((uintptr_t)a.cache | (uintptr_t)a.sblk | (uintptr_t)a.spos | (uintptr_t)a.shead) & 15) == 0;
+  return a.kb >= 2 && a.kb <= 4 && a.vb >= 2 && a.vb <= 4 && (a.flags & V1F_KFP8) == 0 && !((a.flags & V1F_VLM) != 0 && a.vb == 4);
+}
+
 template <int D>
 hipError_t tree_launch(const TreeArgs& a, int64_t tokens, bool vrot, hipStream_t st) {
   const unsigned grid = (unsigned)((int64_t)a.nblk * a.splits * a.B * a.hkv);
   const bool lm = (a.flags & V1F_VLM) != 0 && a.vb == 4;
-  const hipError_t e = lm ? any_launch<D, true>(a, grid, st) : any_launch<D, false>(a, grid, st);
+  const hipError_t e = tree_fast_takes(a) ? (D == 64 ? tree_fast_64(a, grid, st) : D == 128 ? tree_fast_128(a, grid, st) : tree_fast_256(a, grid, st))
+                       : lm ? any_launch<D, true>(a, grid, st) : any_launch<D, false>(a, grid, st);
   if (e != hipSuccess || a.wo == nullptr) return e;
   return tree_merge<D>(a, tokens, vrot, st);
 }

@@ -1,0 +1,317 @@
+// Tree attention for the formats in everyday use: 2-4 bit keys (codebook) with
+// 2-4 bit uniform values, and raw fp16 slots, with 16-bit outputs (float32
+// outputs take the kernel of ftq_tree.hip, whose products are all float32-level).
+//
+// Two LDS buffers of operands: while the waves multiply one tile, each thread
+// turns the bytes of the next, which it loaded a tile earlier, into operands, and
+// requests the bytes of the one after.  One barrier a tile.  A wave takes TK / 4
+// positions of a tile:
+//   K  LPT lanes a position, EK consecutive dims each: pair table lookups, whose
+//      squares give the norm correction, written as 16-byte operands
+//   V  LPQ lanes four positions, DV consecutive dims of each: codes to f16 in
+//      place (mantissa bits, one packed multiply-add), written as the four
+//      positions of each dim, the transposition that the product needs
+// Operands: K table values as f16 (a common scale that keeps their relative
+// errors alike, table_scale), V codes exact (centred, times the scale's own power
+// of two).  bf16 outputs: query and weights as one f16 number, 2^-11 beside the
+// output's 2^-8; fp16 outputs: as hi + lo.
+#pragma once
+
+#include "ftq_internal.h"
+#include "ftq_tree_kernel.h"
+
+namespace ftq {
+
+struct __attribute__((packed, aligned(2))) TreeU32 { uint32_t v; };
+struct __attribute__((packed, aligned(2))) TreeU64 { uint64_t v; };
+
+// Bytes that one lane reads of one position's codes, from an even offset
+template <int N>
+__device__ __forceinline__ void tree_bytes(const uint8_t* p, uint32_t (&w)[(N + 3) / 4]) {
+  if constexpr (N == 1) {
+    w[0] = *p;
+  } else if constexpr (N == 2) {
+    w[0] = *reinterpret_cast<const uint16_t*>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < (N + 3) / 4; i += 2) {
+      if (N - 4 * i > 4) {  // 6 bytes read 8: the slot goes on behind its codes
+        const uint64_t x = reinterpret_cast<const TreeU64*>(p + 4 * i)->v;
+        w[i] = (uint32_t)x;
+        w[i + 1] = (uint32_t)(x >> 32);
+      } else {
+        w[i] = reinterpret_cast<const TreeU32*>(p + 4 * i)->v;
+      }
+    }
+  }
+}
+
+// All waves' LDS accesses before it are done; loads in flight stay in flight
+__device__ __forceinline__ void tree_barrier() { __asm__ volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// KB = TREE_RAW: raw fp16 slots (16-byte aligned)
+template <int D, int KB, int VB>
+struct TreeFmt {
+  using C = TreeGeo<D>;
+  static constexpr bool RAW = KB == TREE_RAW;
+  static constexpr V1Geom G = RAW ? V1Geom{2 * D, 2 * D, 2 * D, 4 * D} : v1_geom(D, KB, VB);
+  static constexpr int TPW = C::TK / 4;                     // positions of a wave
+  static constexpr int LPT = 64 / TPW, EK = D / LPT;        // K: lanes of a position, dims of a lane
+  static constexpr int LPQ = 256 / TPW, DV = D / LPQ;       // V: lanes of four positions, dims of a lane
+  static constexpr int KN = EK * KB / 8;                    // bytes of a lane's K codes
+  static constexpr int VBITS = DV * VB;
+  static constexpr bool VSH = VBITS % 16 != 0 && VBITS != 8;  // V codes that start inside a 16-bit unit
+  static constexpr int VN = VBITS == 8 ? 1 : VSH ? 4 : VBITS / 8;
+  static constexpr int ENTRIES = RAW ? 1 : 1 << (2 * KB);
+  static constexpr float MID = 0.5f * (float)((1 << (RAW ? 0 : VB)) - 1);
+  static constexpr float LIFT = RAW ? 2048.f : 1024.f;      // of the weights' factors, in [1, 2) times this (raw: this)
+
+  uint32_t k[(KN + 3) / 4], v[4][(VN + 3) / 4];
+  uint32_t kn, sm;  // K norm of the lane's position; scale | minimum of V position lane % 4 of its four
+
+  // base: slot of the wave's first position
+  __device__ __forceinline__ void load(const uint8_t* base, uint32_t s_pos, int lane) {
+    const uint8_t* pk = base + (uint32_t)(lane / LPT) * s_pos;
+    const int e = lane % LPT, dq = lane % LPQ;
+    if constexpr (RAW) {
+#pragma unroll
+      for (int i = 0; i < KN / 16; ++i) {
+        const uint4 x = *reinterpret_cast<const uint4*>(pk + e * KN + 16 * i);
+        k[4 * i] = x.x; k[4 * i + 1] = x.y; k[4 * i + 2] = x.z; k[4 * i + 3] = x.w;
+      }
+    } else {
+      tree_bytes<KN>(pk + e * KN, k);
+      kn = *reinterpret_cast<const uint16_t*>(pk + G.mse);
+    }
+    const uint8_t* pv = base + (uint32_t)(lane / LPQ * 4) * s_pos;
+    const uint32_t off = (uint32_t)G.kps + (VBITS == 8 ? dq : (uint32_t)(dq * VBITS) >> 4 << 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (RAW) {
+        if constexpr (VN == 8) {
+          const uint2 x = *reinterpret_cast<const uint2*>(pv + i * s_pos + off);
+          v[i][0] = x.x; v[i][1] = x.y;
+        } else {
+          const uint4 x = *reinterpret_cast<const uint4*>(pv + i * s_pos + off);
+          v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
+        }
+      } else {
+        tree_bytes<VN>(pv + i * s_pos + off, v[i]);
+      }
+    }
+    if constexpr (!RAW) sm = reinterpret_cast<const TreeU32*>(pv + (uint32_t)(dq & 3) * s_pos + G.kps + G.vdb)->v;
+  }
+
+  // To operands of the tile's positions TPW w ..: kb, vb and tb as TreeWave::tile reads them
+  __device__ __forceinline__ void emit(const uint32_t* table, u32x4* kb, u32x4* vb, float (*tb)[C::TK], int w, int lane) const {
+    constexpr int NS = C::NS, NB = C::NB;
+    const int p = w * TPW + lane / LPT, e = lane % LPT, d0 = e * EK;
+    float csq = 0.f;
+#pragma unroll
+    for (int u = 0; u < EK / 8; ++u) {
+      u32x4 x;
+      if constexpr (RAW) {
+        x = u32x4{k[4 * u], k[4 * u + 1], k[4 * u + 2], k[4 * u + 3]};
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[j] = lds_dword_at(table, lut_field<2, 2 * KB>(k, (8 * u + 2 * j) * KB, 0u));
+          const half2_t h = __builtin_bit_cast(half2_t, (uint32_t)x[j]);
+          csq = __builtin_amdgcn_fdot2(h, h, csq, false);
+        }
+      }
+      const int d = d0 + 8 * u;
+      kb[(p >> 4) * NS * 64 + C::kunit(d / 32, p & 15, (d / 8) & 3)] = x;
+    }
+    if constexpr (!RAW) {
+      csq = group_sum<LPT>(csq);
+      if (e == 0) tb[0][p] = f16_bits_to_f32(kn) * __builtin_amdgcn_rsqf(csq + 1e-16f);
+    } else if (e == 0) {
+      tb[0][p] = 1.f;
+    }
+    // V: positions 4 q ..
+    const int q = w * (TPW / 4) + lane / LPQ, dq = lane % LPQ;
+    uint2* out = reinterpret_cast<uint2*>(vb + (q >> 3) * NB * 64 + (q & 3) * 16);
+    const int half = (q >> 2) & 1;
+    auto put = [&](int i, uint32_t lo, uint32_t hi) {  // the lane's dim i, four positions
+      const int d = dq * DV + i, b = d % NB, m = d / NB;
+      out[(b * 64 + m) * 2 + (C::vx(b) ? 1 - half : half)] = make_uint2(lo, hi);
+    };
+    if constexpr (RAW) {
+      // a V that is not finite: operands of 0 and a NaN factor (as tree_any_kernel)
+      uint32_t bad = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int j = 0; j < DV / 2; ++j) any |= ((v[i][j] & 0x7c00u) == 0x7c00u || (v[i][j] & 0x7c000000u) == 0x7c000000u) ? 1u : 0u;
+        const uint64_t lanes = __builtin_amdgcn_ballot_w64(any != 0);
+        constexpr uint64_t ONE = LPQ == 32 ? 0xffffffffull : 0xffffull;
+        bad |= (lanes >> (lane / LPQ * LPQ) & ONE) != 0 ? 1u << i : 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < DV; ++i) {
+        const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
+        uint32_t lo = __builtin_amdgcn_perm(v[1][i / 2], v[0][i / 2], sel), hi = __builtin_amdgcn_perm(v[3][i / 2], v[2][i / 2], sel);
+        lo &= (bad & 1 ? 0u : 0xffffu) | (bad & 2 ? 0u : 0xffff0000u);
+        hi &= (bad & 4 ? 0u : 0xffffu) | (bad & 8 ? 0u : 0xffff0000u);
+        put(i, lo, hi);
+      }
+      if (dq < 4) {
+        tb[1][4 * q + dq] = (bad >> dq) & 1 ? __builtin_nanf("") : LIFT;
+        tb[2][4 * q + dq] = 0.f;
+      }
+    } else {
+      // the lane's own position: scale s = f 2^e with e held where the codes stay
+      // normal and (2^VB + mid) 2^e finite; operand (code - mid) 2^e =
+      // (1 + code 2^-VB) 2^(e + VB) - (2^VB + mid) 2^e
+      const int ex = min(max((int)((sm >> 10) & 31u) - 15, -14), 11);
+      const float sc = f16_bits_to_f32(sm & 0xffffu), mn = f16_bits_to_f32(sm >> 16);
+      if (dq < 4) {
+        tb[1][4 * q + dq] = sc * (__uint_as_float((uint32_t)(127 - ex) << 23) * LIFT);
+        tb[2][4 * q + dq] = __builtin_fmaf(MID, sc, mn);
+      }
+      constexpr uint32_t A = (15u + VB) << 10;  // 2^VB as f16
+      const uint32_t c = __builtin_bit_cast(uint16_t, (_Float16)(-((float)(1 << VB) + MID)));
+      const uint32_t own = ((A + (uint32_t)(ex << 10)) & 0xffffu) | (c + (uint32_t)(ex << 10)) << 16;
+      uint32_t ec[4];  // of the four positions: from the four lanes of a quad
+      ec[0] = (uint32_t)__builtin_amdgcn_mov_dpp((int)own, 0x00, 0xF, 0xF, true);
+      ec[1] = (uint32_t)__builtin_amdgcn_mov_dpp((int)own, 0x55, 0xF, 0xF, true);
+      ec[2] = (uint32_t)__builtin_amdgcn_mov_dpp((int)own, 0xAA, 0xF, 0xF, true);
+      ec[3] = (uint32_t)__builtin_amdgcn_mov_dpp((int)own, 0xFF, 0xF, 0xF, true);
+      const uint32_t vsh = VSH ? (uint32_t)(dq * VBITS) & 15u : 0u;
+      constexpr int PER = 16 / VB;  // codes of a 16-bit window
+      constexpr uint32_t CM = (((1u << VB) - 1u) << (10 - VB)) * 0x10001u;
+#pragma unroll
+      for (int o = 0; o < DV; o += PER) {
+        uint32_t x[2];
+        half2_t e2[2], c2[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t a = v[2 * j][0], b = v[2 * j + 1][0];
+          if constexpr (VSH) {
+            a >>= vsh;
+            b >>= vsh;
+          }
+          if (o * VB == 0) {
+            x[j] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+          } else {
+            const int s = o * VB;
+            x[j] = __builtin_amdgcn_perm(b >> s, a >> s, 0x05040100u);
+          }
+          e2[j] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(ec[2 * j + 1], ec[2 * j], 0x05040100u));
+          c2[j] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(ec[2 * j + 1], ec[2 * j], 0x07060302u));
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          if (o + i >= DV) continue;
+          uint32_t r[2];
+          const int sh = 10 - VB - i * VB;  // the code's bits to the top of the mantissa
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t y = ((sh >= 0 ? x[j] << (sh >= 0 ? sh : 0) : x[j] >> (sh >= 0 ? 0 : -sh)) & CM) | 0x3C003C00u;
+            r[j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2_t, y), e2[j], c2[j]));
+          }
+          put(o + i, r[0], r[1]);
+        }
+      }
+    }
+  }
+};
+
+template <int D, int KB, int VB, int NH>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_fast_kernel(const TreeArgs a) {
+  using C = TreeGeo<D>;
+  using F = TreeFmt<D, KB, VB>;
+  constexpr int CT = C::CT, TK = C::TK, NT = C::NT;
+  using W = TreeWave<D, CT, false, NH, false>;
+  constexpr int BUF = W::KU + W::VU;  // 16-byte units
+  constexpr int QU = 64 * (D + 4) / 4;
+  __shared__ u32x4 pool[2 * BUF > QU ? 2 * BUF : QU];  // operands; before: query rows
+  __shared__ __attribute__((aligned(16))) float tb[2][3][TK];
+  __shared__ uint32_t table[F::ENTRIES];
+  __shared__ int red[4][2];
+
+  const TreeUnit u(a);
+  const int G = a.hq / a.hkv, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (u.blk * 64 * CT >= u.n * G) return;
+
+  if constexpr (!F::RAW) {  // pairs of scaled table values
+    const float sg = table_scale<1 << KB>(a.cent, true).sigma;
+    if (tid < F::ENTRIES)
+      table[tid] = f32_to_f16_bits(sg * a.cent[tid & ((1 << KB) - 1)]) | f32_to_f16_bits(sg * a.cent[tid >> KB]) << 16;
+  }
+  const uint32_t s_pos = (uint32_t)a.spos;
+  // the wave's positions of a tile lie in one run of 16
+  const int sub = wave * F::TPW / 16 * 16, within = wave * F::TPW % 16;
+  const uint8_t* head = a.cache + (int64_t)u.kvh * a.shead + (int64_t)within * a.spos;
+  auto base_of = [&](int pos0, int phys) {  // positions without a page read block 0, and are hidden
+    return head + (int64_t)max(phys, 0) * a.sblk + (int64_t)((pos0 + sub) & ((1 << a.lbs) - 1)) * a.spos;
+  };
+
+  for (int blk = u.blk; blk * 64 * CT < u.n * G; blk += a.nblk) {
+    const int c0 = blk * 64 * CT + wave * 16 * CT;
+    W w;
+    w.columns(a, u, c0, lane);
+    __syncthreads();  // the pool is free
+    w.queries(a, u, c0, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
+    int first, last;
+    w.starts(u.len, lane, wave, red, first, last);
+    first = min(first, u.ctx);  // the tree's own positions always
+    const int held = (int)min((int64_t)u.len, (int64_t)a.max_blocks << a.lbs);  // positions that can have a page
+    const int t0 = first / TK, t1 = max((held + TK - 1) / TK, t0);
+    const int per = (t1 - t0 + a.splits - 1) / a.splits;
+    const int tb0 = t0 + u.split * per, tb1 = min(tb0 + per, t1);
+
+    F raw;
+    int page = -1;  // of the tile after the one in `raw`
+    auto fetch = [&](int t) {  // tile t's bytes, and tile t + 1's page
+      raw.load(base_of(t * TK, page), s_pos, lane);
+      page = t + 1 < tb1 ? tree_page(a, u, (t + 1) * TK + sub) : -1;
+    };
+    if (tb0 < tb1) {
+      page = tree_page(a, u, tb0 * TK + sub);
+      fetch(tb0);
+      raw.emit(table, pool, pool + W::KU, tb[0], wave, lane);
+      if (tb0 + 1 < tb1) fetch(tb0 + 1);
+    }
+    int p = 0;
+    for (int t = tb0; t < tb1; ++t, p ^= 1) {
+      tree_barrier();
+      const int pos0 = t * TK;
+      const u32x4* buf = pool + p * BUF;
+      auto next = [&]() __attribute__((always_inline)) {
+        if (t + 1 < tb1) {
+          raw.emit(table, pool + (p ^ 1) * BUF, pool + (p ^ 1) * BUF + W::KU, tb[p ^ 1], wave, lane);
+          if (t + 2 < tb1) fetch(t + 2);
+        }
+      };
+      const uint32_t on = tree_held<TK>(a, u, pos0);
+      w.tile(a, u, buf, buf + W::KU, tb[p], pos0, pos0 < last || pos0 + TK > u.ctx || on != (1u << NT) - 1u, on, lane, next);
+    }
+    w.finish(a, u, c0, lane, 1.f / F::LIFT);
+  }
+}
+
+template <int D, int KB, int VB>
+hipError_t tree_fast_go(const TreeArgs& a, unsigned grid, hipStream_t st) {
+  if (a.ot == BF16) tree_fast_kernel<D, KB, VB, 1><<<dim3(grid), dim3(256), 0, st>>>(a);
+  else tree_fast_kernel<D, KB, VB, 2><<<dim3(grid), dim3(256), 0, st>>>(a);
+  return hipGetLastError();
+}
+
+template <int D>
+hipError_t tree_fast_launch(const TreeArgs& a, unsigned grid, hipStream_t st) {
+  if (a.kb == TREE_RAW) return tree_fast_go<D, TREE_RAW, TREE_RAW>(a, grid, st);
+#define FTQ_TREE_VB(KB)                                     \
+  return a.vb == 2   ? tree_fast_go<D, KB, 2>(a, grid, st) \
+         : a.vb == 3 ? tree_fast_go<D, KB, 3>(a, grid, st) \
+                     : tree_fast_go<D, KB, 4>(a, grid, st)
+  if (a.kb == 2) FTQ_TREE_VB(2);
+  if (a.kb == 3) FTQ_TREE_VB(3);
+  FTQ_TREE_VB(4);
+#undef FTQ_TREE_VB
+}
+
+}  // namespace ftq

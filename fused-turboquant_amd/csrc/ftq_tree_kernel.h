@@ -19,8 +19,8 @@
 //   V  [32-position tile][block b][part]: dim NB m + b, positions 4 g + j and
 //      16 + 4 g + j (j < 4) -- the rows of the S^T accumulators, so that the weights
 //      go from the score registers into the product without a shuffle
-// and 4 floats a position: K factor, bias (0, or -inf without a page), V factor,
-// V minimum.
+// (with the exchanges of TreeGeo, which spread a dequantising wave's writes over
+// the LDS banks) and 3 floats a position: K factor, V factor, V minimum.
 #pragma once
 
 #include "ftq_attn_dev.h"
@@ -63,6 +63,16 @@ template <int D> struct TreeGeo {
   static constexpr int CT = D == 256 ? 1 : 2;     // 16-column tiles per wave
   static constexpr int TK = D == 64 ? 64 : 32;    // positions of a tile
   static constexpr int NS = D / 32, NB = D / 16, NT = TK / 16, NP = TK / 32;
+  // The dequantising lanes of one position write the steps and rows (s, g) of one m,
+  // which are multiples of 256 bytes apart: m is exchanged with m ^ kx, which differs
+  // among eight lanes that write together.
+  __host__ __device__ static constexpr int kx(int s, int g) {
+    return D == 64 ? 4 * s + 2 * (g >> 1) : D == 128 ? 2 * s + (g >> 1) : s;
+  }
+  __device__ __forceinline__ static int kunit(int ts, int m, int g) { return ts * 64 + g * 16 + (m ^ kx(ts % NS, g)); }
+  // The upper half of the V blocks has the position groups 4 g + j and 16 + 4 g + j
+  // exchanged: two lanes that write blocks NB / 2 apart fill 16 bytes together.
+  __host__ __device__ static constexpr bool vx(int b) { return D != 64 && b >= NB / 2; }
 };
 
 // The sequence, kv head and columns of a workgroup.  Workgroups are dealt to
@@ -112,9 +122,23 @@ __device__ __forceinline__ uint32_t tree_visible(const TreeArgs& a, const TreeUn
   return v | w;
 }
 
-// One wave's columns.  KHL: K as f16 hi + lo; NHP: f16 parts of the weights (the
-// query always has two); VHL: V as hi + lo (Lloyd-Max V).
-template <int D, int CT, bool KHL, int NHP, bool VHL>
+// The block of 16 positions from pos on, or -1 (uniform)
+__device__ __forceinline__ int tree_page(const TreeArgs& a, const TreeUnit& u, int pos) {
+  const int page = pos >> a.lbs;
+  const int phys = pos < u.len && page < a.max_blocks ? a.bt[(int64_t)u.b * a.max_blocks + page] : -1;
+  return phys >= 0 && (int64_t)phys < a.nb ? phys : -1;
+}
+template <int TK>
+__device__ __forceinline__ uint32_t tree_held(const TreeArgs& a, const TreeUnit& u, int pos0) {
+  uint32_t on = 0;
+#pragma unroll
+  for (int k = 0; k < TK / 16; ++k) on |= tree_page(a, u, pos0 + 16 * k) >= 0 ? 1u << k : 0u;
+  return on;
+}
+
+// One wave's columns.  KHL: K as f16 hi + lo; NH: f16 parts of the query and of
+// the weights; VHL: V as hi + lo (Lloyd-Max V).
+template <int D, int CT, bool KHL, int NH, bool VHL>
 struct TreeWave {
   using C = TreeGeo<D>;
   static constexpr int TK = C::TK, NS = C::NS, NB = C::NB, NT = C::NT, NP = C::NP;
@@ -123,7 +147,7 @@ struct TreeWave {
   static constexpr float TAU = 4.f;        // weights stay below 2^TAU
   static constexpr float MINF = -3.0e38f;  // running maximum of a column with no position yet
 
-  half8 qh[CT][NS], ql[CT][NS];
+  half8 qh[CT][NS], ql[NH == 2 ? CT : 1][NH == 2 ? NS : 1];
   float qs[CT];                            // of the scores: 1, or what a query beyond f16's range was divided by
   bool qlarge;                             // some qs is not 1 (wave-uniform)
   float m_run[CT], l_run[CT], z_run[CT];
@@ -145,6 +169,29 @@ struct TreeWave {
 #pragma unroll
       for (int b = 0; b < NB; ++b) acc[ct][b] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
+  }
+
+  // First and last of the columns' first context positions over the workgroup, `none` for a wave without columns
+  __device__ __forceinline__ void starts(int none, int lane, int wave, int (*red)[2], int& first, int& last) const {
+    first = none;
+    last = 0;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+      if (live[ct]) {
+        first = min(first, start[ct]);
+        last = max(last, start[ct]);
+      }
+    first = (int)wave_min_u32((uint32_t)first);
+    last = (int)~wave_min_u32(~(uint32_t)last);
+    if (lane == 0) {
+      red[wave][0] = first;
+      red[wave][1] = last;
+    }
+    __syncthreads();
+    first = min(min(red[0][0], red[1][0]), min(red[2][0], red[3][0]));
+    last = max(max(red[0][1], red[1][1]), max(red[2][1], red[3][1]));
+    first = __builtin_amdgcn_readfirstlane(first);
+    last = __builtin_amdgcn_readfirstlane(last);
   }
 
   // The columns' queries, rotated and scaled, as f16 hi + lo.  One query per 16
@@ -205,7 +252,7 @@ struct TreeWave {
         for (int j = 0; j < 4; ++j) {
           const float x = rows[n][32 * s + 8 * g + 2 * j], y = rows[n][32 * s + 8 * g + 2 * j + 1];
           h[j] = pk_f16(x, y);
-          l[j] = pk_f16(f16_rest(x, h[j], 0), f16_rest(y, h[j], 1));
+          l[j] = NH == 2 ? pk_f16(f16_rest(x, h[j], 0), f16_rest(y, h[j], 1)) : 0u;
         }
         hi[s] = __builtin_bit_cast(half8, u32x4{h[0], h[1], h[2], h[3]});
         lo[s] = __builtin_bit_cast(half8, u32x4{l[0], l[1], l[2], l[3]});
@@ -218,19 +265,20 @@ struct TreeWave {
 #pragma unroll
           for (int s = 0; s < NS; ++s) {
             qh[c][s] = hi[s];
-            ql[c][s] = lo[s];
+            if constexpr (NH == 2) ql[c][s] = lo[s];
           }
         }
       qlarge = qlarge || __builtin_amdgcn_ballot_w64(inv != 1.f) != 0;
     }
   }
 
-  // One tile: kb, vb its operands, tb its factors.  vis: bits of the positions
-  // that each column attends (edge tiles only).  next(): called once this tile's
-  // operands are in registers.
-  template <bool EDGE, typename F>
-  __device__ __forceinline__ void tile(const u32x4* kb, const u32x4* vb, const float (*tb)[TK], const uint32_t (&vis)[CT][NP],
-                                       int lane, F next) {
+  // One tile of the positions from pos0 on: kb, vb its operands ([k][part][NS] and
+  // [p][part][NB] units of 64), tb its factors.  edge (uniform): some column does not
+  // attend all of it, or (bit k of `on`: positions 16 k .. have a page) nobody some.
+  // next(): called behind the reads of the K operands.
+  template <typename F>
+  __device__ __forceinline__ void tile(const TreeArgs& a, const TreeUnit& u, const u32x4* kb, const u32x4* vb,
+                                       const float (*tb)[TK], int pos0, bool edge, uint32_t on, int lane, F next) {
     const int g = lane >> 4;
     floatx4 s[NT][CT];
 #pragma unroll
@@ -242,14 +290,17 @@ struct TreeWave {
       half8 xh[NT], xl[NT];
 #pragma unroll
       for (int k = 0; k < NT; ++k) {
-        xh[k] = __builtin_bit_cast(half8, kb[((k * NS + d) * KP) * 64 + lane]);
-        if constexpr (KHL) xl[k] = __builtin_bit_cast(half8, kb[((k * NS + d) * KP + 1) * 64 + lane]);
+        const int at = C::kunit(d, lane & 15, g);
+        xh[k] = __builtin_bit_cast(half8, kb[(k * KP) * NS * 64 + at]);
+        if constexpr (KHL) xl[k] = __builtin_bit_cast(half8, kb[(k * KP + 1) * NS * 64 + at]);
       }
       // the low products first: what they add is not lost beside the high ones' sum
+      if constexpr (NH == 2) {
 #pragma unroll
-      for (int k = 0; k < NT; ++k)
+        for (int k = 0; k < NT; ++k)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[k], ql[ct][d], s[k][ct], 0, 0, 0);
+          for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[k], ql[ct][d], s[k][ct], 0, 0, 0);
+      }
       if constexpr (KHL) {
 #pragma unroll
         for (int k = 0; k < NT; ++k)
@@ -261,18 +312,17 @@ struct TreeWave {
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[k], qh[ct][d], s[k][ct], 0, 0, 0);
     }
-    half8 xv[NP * NB];
-#pragma unroll
-    for (int i = 0; i < NP * NB; ++i) xv[i] = __builtin_bit_cast(half8, vb[i * VP * 64 + lane]);
-    float tf[NT][4][4];  // the factors of this lane's positions 16 k + 4 g + i
+    __builtin_amdgcn_sched_barrier(0);  // the next tile's operands are not formed beside this one's reads (registers)
+    next();
+    __builtin_amdgcn_sched_barrier(0);
+    float tf[NT][3][4];  // the factors of this lane's positions 16 k + 4 g + i
 #pragma unroll
     for (int k = 0; k < NT; ++k)
 #pragma unroll
-      for (int f = 0; f < 4; ++f) {
+      for (int f = 0; f < 3; ++f) {
         const float4 x = *reinterpret_cast<const float4*>(&tb[f][16 * k + 4 * g]);
         tf[k][f][0] = x.x; tf[k][f][1] = x.y; tf[k][f][2] = x.z; tf[k][f][3] = x.w;
       }
-    next();
     if (qlarge) {
 #pragma unroll
       for (int k = 0; k < NT; ++k)
@@ -284,15 +334,21 @@ struct TreeWave {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[k][ct][i] = __builtin_fmaf(s[k][ct][i], tf[k][0][i], tf[k][1][i]);
-    if constexpr (EDGE) {
+        for (int i = 0; i < 4; ++i) s[k][ct][i] *= tf[k][0][i];
+    if (edge) {
 #pragma unroll
-      for (int k = 0; k < NT; ++k)
+      for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
+        for (int p = 0; p < NP; ++p) {
+          const uint32_t held = ((on >> (2 * p)) & 1u ? 0xffffu : 0u) | ((on >> (2 * p + 1)) & 1u ? 0xffff0000u : 0u);
+          uint32_t vis = live[ct] ? tree_visible(a, u, tok[ct], row[ct], start[ct], pos0 + 32 * p) & held : 0u;
+          vis >>= 4 * g;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (((vis[ct][k >> 1] >> (16 * (k & 1) + 4 * g + i)) & 1u) == 0) s[k][ct][i] = -INFINITY;
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (((vis >> (16 * k + i)) & 1u) == 0) s[2 * p + k][ct][i] = -INFINITY;
+        }
     }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
@@ -314,49 +370,52 @@ struct TreeWave {
     }
     // weights: p; p x V minimum kept aside; p x V factor as f16 parts.  A tile's
     // sums are formed first, so that many small weights beside a large one count.
-    u32x4 ph[NP][CT], pl[NP][CT];
+    u32x4 ph[NP][CT], pl[NH == 2 ? NP : 1][NH == 2 ? CT : 1];
+    auto weights = [&](auto masked) __attribute__((always_inline)) {
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      float lt = 0.f, zt = 0.f;
+      for (int ct = 0; ct < CT; ++ct) {
+        float lt = 0.f, zt = 0.f;
 #pragma unroll
-      for (int k = 0; k < NT; ++k) {
-        float w[4];
+        for (int k = 0; k < NT; ++k) {
+          float w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool hid = EDGE && s[k][ct][i] == -INFINITY;  // its factors may be infinite or NaN
-          const float e = __builtin_amdgcn_exp2f(s[k][ct][i] - m_run[ct]);
-          lt += e;
-          zt = __builtin_fmaf(e, hid ? 0.f : tf[k][3][i], zt);
-          w[i] = e * (hid ? 0.f : tf[k][2][i]);
+          for (int i = 0; i < 4; ++i) {
+            const bool hid = decltype(masked)::value && s[k][ct][i] == -INFINITY;  // its factors may be infinite or NaN
+            const float e = __builtin_amdgcn_exp2f(s[k][ct][i] - m_run[ct]);
+            lt += e;
+            zt = __builtin_fmaf(e, hid ? 0.f : tf[k][2][i], zt);
+            w[i] = e * (hid ? 0.f : tf[k][1][i]);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t hi = pk_f16(w[2 * h], w[2 * h + 1]);
+            ph[k >> 1][ct][2 * (k & 1) + h] = hi;
+            if constexpr (NH == 2) pl[k >> 1][ct][2 * (k & 1) + h] = pk_f16(f16_rest(w[2 * h], hi, 0), f16_rest(w[2 * h + 1], hi, 1));
+          }
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t hi = pk_f16(w[2 * h], w[2 * h + 1]);
-          ph[k >> 1][ct][2 * (k & 1) + h] = hi;
-          if constexpr (NHP == 2) pl[k >> 1][ct][2 * (k & 1) + h] = pk_f16(f16_rest(w[2 * h], hi, 0), f16_rest(w[2 * h + 1], hi, 1));
-        }
+        l_run[ct] += lt;
+        z_run[ct] += zt;
       }
-      l_run[ct] += lt;
-      z_run[ct] += zt;
-    }
+    };
+    if (edge) weights(std::true_type{});
+    else weights(std::false_type{});
+    auto of = [](const u32x4& w, int b) { return __builtin_bit_cast(half8, C::vx(b) ? u32x4{w[2], w[3], w[0], w[1]} : w); };
 #pragma unroll
     for (int p = 0; p < NP; ++p)
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
+        const half8 x = __builtin_bit_cast(half8, vb[(p * VP * NB + b) * 64 + lane]);
         if constexpr (VHL) {
-          const half8 x = __builtin_bit_cast(half8, vb[((p * NB + b) * VP + 1) * 64 + lane]);
+          const half8 y = __builtin_bit_cast(half8, vb[((p * VP + 1) * NB + b) * 64 + lane]);
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-            acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(half8, ph[p][ct]), acc[ct][b], 0, 0, 0);
+          for (int ct = 0; ct < CT; ++ct) acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, of(ph[p][ct], b), acc[ct][b], 0, 0, 0);
         }
-        if constexpr (NHP == 2) {
+        if constexpr (NH == 2) {
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-            acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xv[p * NB + b], __builtin_bit_cast(half8, pl[p][ct]), acc[ct][b], 0, 0, 0);
+          for (int ct = 0; ct < CT; ++ct) acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, of(pl[p][ct], b), acc[ct][b], 0, 0, 0);
         }
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-          acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xv[p * NB + b], __builtin_bit_cast(half8, ph[p][ct]), acc[ct][b], 0, 0, 0);
+        for (int ct = 0; ct < CT; ++ct) acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, of(ph[p][ct], b), acc[ct][b], 0, 0, 0);
       }
   }
 

@@ -40,12 +40,6 @@ __device__ __forceinline__ float pow2_of(float mx) {
   return __uint_as_float((uint32_t)min(max(254 - e, 1), 253) << 23);
 }
 
-// The weights' factors (V scale without its own power of two, which is in the V
-// operand) times this: with 2^TAU = 16 the largest weight is 16 * 2 * LIFT <= 2^15,
-// and its low part is a normal f16 number as far down as f16 has them.  Raw slots
-// have a factor of 1.
-__host__ __device__ constexpr float tree_lift(bool raw) { return raw ? 2048.f : 1024.f; }
-
 // Any slot format: the tile's slots as rows of LDS, from them the factors of each
 // position, then the operands.  Every product is float32-level (hi + lo parts of
 // what f16 does not hold exactly).  Bound by the LDS reads and bit extractions of
@@ -57,10 +51,11 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
   using W = TreeWave<D, CT, true, 2, LM>;
   constexpr int LPT = 256 / TK, DPL = D / LPT;  // lanes of a position, their dims
   extern __shared__ __attribute__((aligned(16))) uint32_t pool[];  // slots [TK][pitch]; before: query rows; both: operands behind
-  __shared__ __attribute__((aligned(16))) float tb[3][TK];
+  __shared__ __attribute__((aligned(16))) float tb[2][TK];
+  __shared__ u32x4 xb[NP * 64];
   __shared__ uint32_t tabk[256], tabv[16];  // f16 hi | lo << 16 of the scaled table
   __shared__ float tabn[256];
-  __shared__ float vex[TK];                 // 2^e of the position's V operand
+  __shared__ float vex[TK];                 // multiplier of the position's V operand
   __shared__ float table_scale_inv;
   __shared__ int red[4][2];
 
@@ -74,6 +69,7 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
   u32x4* kf = reinterpret_cast<u32x4*>(pool + (TK * pitch + 3) / 4 * 4);
   u32x4* vf = kf + W::KU;
   const float mid = raw ? 0.f : 0.5f * (float)((1 << a.vb) - 1);
+  for (int i = tid; i < NP * 64; i += 256) xb[i] = u32x4{0, 0, 0, 0};
 
   if (!raw && wave == 0) {  // tables
     const int nk = 1 << a.kb;
@@ -98,11 +94,10 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
   for (int blk = u.blk; blk * 64 * CT < u.n * G; blk += a.nblk) {
     const int c0 = blk * 64 * CT + wave * 16 * CT;
     W w;
-    w.columns(a, u, c0, lane);
-    __syncthreads();  // the pool is free (and the tables written)
-    w.queries(a, u, c0, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
     int first, last;
-    w.starts(u.len, lane, wave, red, first, last);
+    w.columns(a, u, c0, lane, wave, red, u.len, first, last);  // its barrier: the pool is free, and the tables written
+    w.queries(a, u, c0, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
+    __syncthreads();
     first = min(first, u.ctx);  // the tree's own positions always
     const int held = (int)min((int64_t)u.len, (int64_t)a.max_blocks << a.lbs);  // positions that can have a page
     const int t0 = first / TK, t1 = max((held + TK - 1) / TK, t0);
@@ -146,27 +141,26 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
         }
         if (raw) beyond = group_sum<LPT>(beyond);
         if (sub == 0) {
-          // A raw V that is not finite: operands of 0 and a NaN factor, so that the
-          // rows that attend it are NaN and those that only meet it with a weight of
-          // 0 are not.
-          float fk = 1.f, vs = beyond == 0.f ? tree_lift(true) : __builtin_nanf(""), vm = 0.f, ve = beyond == 0.f ? 1.f : 0.f;
+          // A raw V that is not finite (as a scale or minimum): operands of 0 and a NaN
+          // factor, so that the rows that attend it are NaN and the others, whose
+          // products meet it with a weight of 0, are not.
+          float fk = 1.f;
+          TreeV v{beyond == 0.f ? TREE_LIFT : __builtin_nanf(""), beyond == 0.f ? 1.f : 0.f, beyond == 0.f ? tree_parts(32.f) : 0u, 0u};
           if (!raw) {
             if (!kf8) fk = f16_bits_to_f32(row_bits(row, 8 * geo.mse, 16)) / __builtin_sqrtf(csq + 1e-16f) * table_scale_inv;
-            const uint32_t sb = row_bits(row, 8 * (geo.kps + geo.vdb), 16);
-            float sc = f16_bits_to_f32(sb);
-            if constexpr (LM) sc = sc / __builtin_sqrtf(vsq + 1e-16f) * (512.f * table_scale_inv);
-            // V operand times 2^e, e the scale's own exponent, held where the largest
-            // operand stays finite (codes: 128 at most, 2^e <= 2^8; a Lloyd-Max value:
-            // below 2) and the factor an ordinary number
-            const int e = min(max((int)((__float_as_uint(sc) >> 23) & 255u) - 127, -14), LM ? 14 : a.vb == 8 ? 8 : 12);
-            ve = __uint_as_float((uint32_t)(127 + e) << 23);
-            vs = sc * __uint_as_float((uint32_t)(127 - e) << 23) * tree_lift(false);
-            if (!LM) vm = __builtin_fmaf(mid, sc, f16_bits_to_f32(row_bits(row, 8 * (geo.kps + geo.vdb) + 16, 16)));
+            float sc = f16_bits_to_f32(row_bits(row, 8 * (geo.kps + geo.vdb), 16)), vm = 0.f;
+            if constexpr (LM) sc = sc / __builtin_sqrtf(vsq + 1e-16f) * (512.f * table_scale_inv);  // the norm's
+            else vm = __builtin_fmaf(mid, sc, f16_bits_to_f32(row_bits(row, 8 * (geo.kps + geo.vdb) + 16, 16)));
+            // (codes of 128 at most times 2^8; Lloyd-Max values are below 2)
+            v = tree_v(sc, vm, LM ? 14 : a.vb == 8 ? 8 : 11);
           }
           tb[0][p] = fk;
-          tb[1][p] = vs;
-          tb[2][p] = vm;
-          vex[p] = ve;
+          tb[1][p] = v.f;
+          *tree_x<D>(xb, p, 0) = (uint16_t)v.x;
+          *tree_x<D>(xb, p, 1) = (uint16_t)(v.x >> 16);
+          *tree_x<D>(xb, p, 2) = (uint16_t)v.y;
+          *tree_x<D>(xb, p, 3) = (uint16_t)(v.y >> 16);
+          vex[p] = v.mult;
         }
       }
       __syncthreads();
@@ -219,10 +213,10 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
       }
       __syncthreads();
       const uint32_t on = tree_held<TK>(a, u, pos0);  // bit k: positions 16 k .. of the tile have a page
-      w.tile(a, u, kf, vf, tb, pos0, pos0 < last || pos0 + TK > u.ctx || on != (1u << NT) - 1u, on, lane, [] {});
+      w.tile(a, u, kf, vf, xb, tb, pos0, pos0 < last || pos0 + TK > u.ctx || on != (1u << NT) - 1u, on, lane, [] {});
       __syncthreads();  // before the next tile's rows
     }
-    w.finish(a, u, c0, lane, 1.f / tree_lift(raw));
+    w.finish(a, u, c0, lane);
   }
 }
 

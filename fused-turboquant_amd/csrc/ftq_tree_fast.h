@@ -49,6 +49,12 @@ __device__ __forceinline__ void tree_bytes(const uint8_t* p, uint32_t (&w)[(N + 
 // All waves' LDS accesses before it are done; loads in flight stay in flight
 __device__ __forceinline__ void tree_barrier() { __asm__ volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// A tile's operands: 16-byte units of K, V, X and the factors
+template <int D> struct TreeBuf {
+  using C = TreeGeo<D>;
+  static constexpr int V = C::NT * C::NS * 64, X = V + C::NP * C::NB * 64, T = X + C::NP * 64, SIZE = T + 2 * C::TK / 4;
+};
+
 // KB = TREE_RAW: raw fp16 slots (16-byte aligned)
 template <int D, int KB, int VB>
 struct TreeFmt {
@@ -64,46 +70,48 @@ struct TreeFmt {
   static constexpr int VN = VBITS == 8 ? 1 : VSH ? 4 : VBITS / 8;
   static constexpr int ENTRIES = RAW ? 1 : 1 << (2 * KB);
   static constexpr float MID = 0.5f * (float)((1 << (RAW ? 0 : VB)) - 1);
-  static constexpr float LIFT = RAW ? 2048.f : 1024.f;      // of the weights' factors, in [1, 2) times this (raw: this)
 
   uint32_t k[(KN + 3) / 4], v[4][(VN + 3) / 4];
   uint32_t kn, sm;  // K norm of the lane's position; scale | minimum of V position lane % 4 of its four
 
-  // base: slot of the wave's first position
+  // base: slot of the wave's first position (uniform)
   __device__ __forceinline__ void load(const uint8_t* base, uint32_t s_pos, int lane) {
-    const uint8_t* pk = base + (uint32_t)(lane / LPT) * s_pos;
     const int e = lane % LPT, dq = lane % LPQ;
+    const uint32_t ko = (uint32_t)(lane / LPT) * s_pos, vo = (uint32_t)(lane / LPQ * 4) * s_pos;
+    const uint32_t off = vo + (uint32_t)G.kps + (VBITS == 8 ? dq : (uint32_t)(dq * VBITS) >> 4 << 1);
     if constexpr (RAW) {
 #pragma unroll
       for (int i = 0; i < KN / 16; ++i) {
-        const uint4 x = *reinterpret_cast<const uint4*>(pk + e * KN + 16 * i);
+        const uint4 x = *reinterpret_cast<const uint4*>(base + (ko + e * KN) + 16 * i);
         k[4 * i] = x.x; k[4 * i + 1] = x.y; k[4 * i + 2] = x.z; k[4 * i + 3] = x.w;
       }
     } else {
-      tree_bytes<KN>(pk + e * KN, k);
-      kn = *reinterpret_cast<const uint16_t*>(pk + G.mse);
+      tree_bytes<KN>(base + (ko + e * KN), k);
+      kn = *reinterpret_cast<const uint16_t*>(base + ko + G.mse);
     }
-    const uint8_t* pv = base + (uint32_t)(lane / LPQ * 4) * s_pos;
-    const uint32_t off = (uint32_t)G.kps + (VBITS == 8 ? dq : (uint32_t)(dq * VBITS) >> 4 << 1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      const uint8_t* pv = base + (int64_t)i * s_pos;  // uniform
       if constexpr (RAW) {
         if constexpr (VN == 8) {
-          const uint2 x = *reinterpret_cast<const uint2*>(pv + i * s_pos + off);
+          const uint2 x = *reinterpret_cast<const uint2*>(pv + off);
           v[i][0] = x.x; v[i][1] = x.y;
         } else {
-          const uint4 x = *reinterpret_cast<const uint4*>(pv + i * s_pos + off);
+          const uint4 x = *reinterpret_cast<const uint4*>(pv + off);
           v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
         }
       } else {
-        tree_bytes<VN>(pv + i * s_pos + off, v[i]);
+        tree_bytes<VN>(pv + off, v[i]);
       }
     }
-    if constexpr (!RAW) sm = reinterpret_cast<const TreeU32*>(pv + (uint32_t)(dq & 3) * s_pos + G.kps + G.vdb)->v;
+    if constexpr (!RAW) sm = reinterpret_cast<const TreeU32*>(base + (vo + (uint32_t)(dq & 3) * s_pos) + (G.kps + G.vdb))->v;
   }
 
-  // To operands of the tile's positions TPW w ..: kb, vb and tb as TreeWave::tile reads them
-  __device__ __forceinline__ void emit(const uint32_t* table, u32x4* kb, u32x4* vb, float (*tb)[C::TK], int w, int lane) const {
+  // To operands of the tile's positions TPW w .., in a buffer
+  __device__ __forceinline__ void emit(const uint32_t* table, u32x4* buf, int w, int lane) const {
+    using B = TreeBuf<D>;
+    u32x4 *kb = buf, *vb = buf + B::V, *xb = buf + B::X;
+    float(*tb)[C::TK] = reinterpret_cast<float(*)[C::TK]>(buf + B::T);
     constexpr int NS = C::NS, NB = C::NB;
     const int p = w * TPW + lane / LPT, e = lane % LPT, d0 = e * EK;
     float csq = 0.f;
@@ -158,27 +166,30 @@ struct TreeFmt {
         put(i, lo, hi);
       }
       if (dq < 4) {
-        tb[1][4 * q + dq] = (bad >> dq) & 1 ? __builtin_nanf("") : LIFT;
-        tb[2][4 * q + dq] = 0.f;
+        const bool b = (bad >> dq) & 1;
+        tb[1][4 * q + dq] = b ? __builtin_nanf("") : TREE_LIFT;
+        *tree_x<D>(xb, 4 * q + dq, 0) = b ? 0 : 0x5000;  // 32
       }
     } else {
-      // the lane's own position: scale s = f 2^e with e held where the codes stay
-      // normal and (2^VB + mid) 2^e finite; operand (code - mid) 2^e =
-      // (1 + code 2^-VB) 2^(e + VB) - (2^VB + mid) 2^e
-      const int ex = min(max((int)((sm >> 10) & 31u) - 15, -14), 11);
-      const float sc = f16_bits_to_f32(sm & 0xffffu), mn = f16_bits_to_f32(sm >> 16);
+      // the lane's own position; operand (code - mid) mult = (1 + code 2^-VB) 2^VB mult
+      // - (2^VB + mid) mult
+      const float sc = f16_bits_to_f32(sm & 0xffffu);
+      const TreeV r = tree_v(sc, __builtin_fmaf(MID, sc, f16_bits_to_f32(sm >> 16)), 11);
       if (dq < 4) {
-        tb[1][4 * q + dq] = sc * (__uint_as_float((uint32_t)(127 - ex) << 23) * LIFT);
-        tb[2][4 * q + dq] = __builtin_fmaf(MID, sc, mn);
+        tb[1][4 * q + dq] = r.f;
+        *tree_x<D>(xb, 4 * q + dq, 0) = (uint16_t)r.x;
+        *tree_x<D>(xb, 4 * q + dq, 1) = (uint16_t)(r.x >> 16);
+        *tree_x<D>(xb, 4 * q + dq, 2) = (uint16_t)r.y;
+        *tree_x<D>(xb, 4 * q + dq, 3) = (uint16_t)(r.y >> 16);
       }
-      constexpr uint32_t A = (15u + VB) << 10;  // 2^VB as f16
-      const uint32_t c = __builtin_bit_cast(uint16_t, (_Float16)(-((float)(1 << VB) + MID)));
-      const uint32_t own = ((A + (uint32_t)(ex << 10)) & 0xffffu) | (c + (uint32_t)(ex << 10)) << 16;
+      const uint32_t own = pk_f16(r.mult * (float)(1 << VB), r.mult * -((float)(1 << VB) + MID));
       uint32_t ec[4];  // of the four positions: from the four lanes of a quad
       ec[0] = (uint32_t)__builtin_amdgcn_mov_dpp((int)own, 0x00, 0xF, 0xF, true);
       ec[1] = (uint32_t)__builtin_amdgcn_mov_dpp((int)own, 0x55, 0xF, 0xF, true);
       ec[2] = (uint32_t)__builtin_amdgcn_mov_dpp((int)own, 0xAA, 0xF, 0xF, true);
       ec[3] = (uint32_t)__builtin_amdgcn_mov_dpp((int)own, 0xFF, 0xF, 0xF, true);
+      uint32_t one = 0x3C003C00u;
+      asm("" : "+v"(one));  // in a register: the mask and it then are one v_and_or_b32
       const uint32_t vsh = VSH ? (uint32_t)(dq * VBITS) & 15u : 0u;
       constexpr int PER = 16 / VB;  // codes of a 16-bit window
       constexpr uint32_t CM = (((1u << VB) - 1u) << (10 - VB)) * 0x10001u;
@@ -209,7 +220,7 @@ struct TreeFmt {
           const int sh = 10 - VB - i * VB;  // the code's bits to the top of the mantissa
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const uint32_t y = ((sh >= 0 ? x[j] << (sh >= 0 ? sh : 0) : x[j] >> (sh >= 0 ? 0 : -sh)) & CM) | 0x3C003C00u;
+            const uint32_t y = ((sh >= 0 ? x[j] << (sh >= 0 ? sh : 0) : x[j] >> (sh >= 0 ? 0 : -sh)) & CM) | one;
             r[j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2_t, y), e2[j], c2[j]));
           }
           put(o + i, r[0], r[1]);
@@ -220,15 +231,14 @@ struct TreeFmt {
 };
 
 template <int D, int KB, int VB, int NH>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_fast_kernel(const TreeArgs a) {
+__global__ __launch_bounds__(256, 2) void tree_fast_kernel(const TreeArgs a) {
   using C = TreeGeo<D>;
   using F = TreeFmt<D, KB, VB>;
-  constexpr int CT = C::CT, TK = C::TK, NT = C::NT;
+  constexpr int CT = C::CT, TK = C::TK, NT = C::NT, NP = C::NP;
   using W = TreeWave<D, CT, false, NH, false>;
-  constexpr int BUF = W::KU + W::VU;  // 16-byte units
+  using B = TreeBuf<D>;
   constexpr int QU = 64 * (D + 4) / 4;
-  __shared__ u32x4 pool[2 * BUF > QU ? 2 * BUF : QU];  // operands; before: query rows
-  __shared__ __attribute__((aligned(16))) float tb[2][3][TK];
+  __shared__ u32x4 pool[2 * B::SIZE > QU ? 2 * B::SIZE : QU];  // two buffers; before: query rows
   __shared__ uint32_t table[F::ENTRIES];
   __shared__ int red[4][2];
 
@@ -243,21 +253,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_fast_kernel(const 
       table[tid] = f32_to_f16_bits(sg * a.cent[tid & ((1 << KB) - 1)]) | f32_to_f16_bits(sg * a.cent[tid >> KB]) << 16;
   }
   const uint32_t s_pos = (uint32_t)a.spos;
+  const int nb32 = (int)min(a.nb, (int64_t)0x7fffffff);
   // the wave's positions of a tile lie in one run of 16
-  const int sub = wave * F::TPW / 16 * 16, within = wave * F::TPW % 16;
+  const int sub = wave * F::TPW / 16, within = wave * F::TPW % 16;
   const uint8_t* head = a.cache + (int64_t)u.kvh * a.shead + (int64_t)within * a.spos;
-  auto base_of = [&](int pos0, int phys) {  // positions without a page read block 0, and are hidden
-    return head + (int64_t)max(phys, 0) * a.sblk + (int64_t)((pos0 + sub) & ((1 << a.lbs) - 1)) * a.spos;
-  };
 
   for (int blk = u.blk; blk * 64 * CT < u.n * G; blk += a.nblk) {
     const int c0 = blk * 64 * CT + wave * 16 * CT;
     W w;
-    w.columns(a, u, c0, lane);
-    __syncthreads();  // the pool is free
-    w.queries(a, u, c0, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
     int first, last;
-    w.starts(u.len, lane, wave, red, first, last);
+    w.columns(a, u, c0, lane, wave, red, u.len, first, last);  // its barrier: the pool is free
+    w.queries(a, u, c0, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
+    __syncthreads();
+    if (tid < 2 * 64 * NP) pool[tid / (64 * NP) * B::SIZE + B::X + tid % (64 * NP)] = u32x4{0, 0, 0, 0};
+    __syncthreads();
     first = min(first, u.ctx);  // the tree's own positions always
     const int held = (int)min((int64_t)u.len, (int64_t)a.max_blocks << a.lbs);  // positions that can have a page
     const int t0 = first / TK, t1 = max((held + TK - 1) / TK, t0);
@@ -265,32 +274,47 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_fast_kernel(const 
     const int tb0 = t0 + u.split * per, tb1 = min(tb0 + per, t1);
 
     F raw;
-    int page = -1;  // of the tile after the one in `raw`
-    auto fetch = [&](int t) {  // tile t's bytes, and tile t + 1's page
-      raw.load(base_of(t * TK, page), s_pos, lane);
-      page = t + 1 < tb1 ? tree_page(a, u, (t + 1) * TK + sub) : -1;
+    // Block-table entries of the tile to load next, lane k: positions 16 k ..; a
+    // vector load in line with the slots', so that nothing waits for it alone
+    int entry = -1;
+    uint32_t on = 0;  // runs of 16 with a page, of the tile in `raw`
+    const int32_t* bt = a.bt + (int64_t)u.b * a.max_blocks;
+    auto entries = [&](int t) __attribute__((always_inline)) {
+      const int pos = t * TK + 16 * (lane & (NT - 1)), at = pos >> a.lbs;
+      entry = pos < u.len && at < a.max_blocks ? bt[at] : -1;
     };
+    auto fetch = [&](int t) __attribute__((always_inline)) {  // tile t's bytes, and the next one's entries
+      const bool ok = (uint32_t)entry < (uint32_t)nb32;
+      on = (uint32_t)__builtin_amdgcn_ballot_w64(ok) & ((1u << NT) - 1u);
+      const int page = __builtin_amdgcn_readlane(ok ? entry : 0, sub);  // positions without one read block 0
+      const int64_t at = (int64_t)page * a.sblk + (int64_t)((t * TK + 16 * sub) & ((1 << a.lbs) - 1)) * a.spos;
+      raw.load(head + at, s_pos, lane);
+      entries(t + 1);
+    };
+    uint32_t on_now = 0;
     if (tb0 < tb1) {
-      page = tree_page(a, u, tb0 * TK + sub);
+      entries(tb0);
       fetch(tb0);
-      raw.emit(table, pool, pool + W::KU, tb[0], wave, lane);
+      raw.emit(table, pool, wave, lane);
+      on_now = on;
       if (tb0 + 1 < tb1) fetch(tb0 + 1);
     }
     int p = 0;
     for (int t = tb0; t < tb1; ++t, p ^= 1) {
       tree_barrier();
       const int pos0 = t * TK;
-      const u32x4* buf = pool + p * BUF;
+      const u32x4* buf = pool + p * B::SIZE;
+      const uint32_t now = on_now;
       auto next = [&]() __attribute__((always_inline)) {
         if (t + 1 < tb1) {
-          raw.emit(table, pool + (p ^ 1) * BUF, pool + (p ^ 1) * BUF + W::KU, tb[p ^ 1], wave, lane);
+          raw.emit(table, pool + (p ^ 1) * B::SIZE, wave, lane);
+          on_now = on;
           if (t + 2 < tb1) fetch(t + 2);
         }
       };
-      const uint32_t on = tree_held<TK>(a, u, pos0);
-      w.tile(a, u, buf, buf + W::KU, tb[p], pos0, pos0 < last || pos0 + TK > u.ctx || on != (1u << NT) - 1u, on, lane, next);
+      w.tile(a, u, buf, buf + B::V, buf + B::X, reinterpret_cast<const float(*)[TK]>(buf + B::T), pos0, pos0 < last || pos0 + TK > u.ctx || now != (1u << NT) - 1u, now, lane, next);
     }
-    w.finish(a, u, c0, lane, 1.f / F::LIFT);
+    w.finish(a, u, c0, lane);
   }
 }
 

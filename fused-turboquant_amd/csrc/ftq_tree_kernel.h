@@ -10,6 +10,12 @@
 // matrix-core operands, and every wave reads these for its 16 CT columns:
 //   S^T = K Q^T, softmax in the log2 domain with a lazily raised maximum,
 //   O^T = V^T P^T (v_mfma_f32_16x16x32_f16, float32 sums).
+// With a position's V = (code - mid) scale + (min + mid scale), the weight enters
+// the product as w = p f, f the scale without the power of two that its operand
+// (code - mid) 2^e carries, and the sums of the weights and of the minima are four
+// more rows of it, 1 / f and (min + mid scale) / f in two parts each: two matrix
+// instructions in place of 32 additions, and the rounding of w is in numerator and
+// denominator alike.
 // The context is split over workgroups where the columns alone do not fill the
 // GPU, and the parts meet in merge_splits_kernel.
 //
@@ -19,8 +25,10 @@
 //   V  [32-position tile][block b][part]: dim NB m + b, positions 4 g + j and
 //      16 + 4 g + j (j < 4) -- the rows of the S^T accumulators, so that the weights
 //      go from the score registers into the product without a shuffle
-// (with the exchanges of TreeGeo, which spread a dequantising wave's writes over
-// the LDS banks) and 3 floats a position: K factor, V factor, V minimum.
+//   X  [32-position tile]: rows 0 .. 3 the parts of 1 / f and of the minimum, the
+//      others 0, positions as V
+// (K and V with the exchanges of TreeGeo, which spread a dequantising wave's writes
+// over the LDS banks) and 2 floats a position: K factor, weight factor f LIFT.
 #pragma once
 
 #include "ftq_attn_dev.h"
@@ -97,18 +105,19 @@ struct TreeUnit {
   }
 };
 
-// Bits of row t's mask (null: tokens up to row r of its own) for the 32 positions from
-// pos0 on, the context's from `start` on among them.
-__device__ __forceinline__ uint32_t tree_visible(const TreeArgs& a, const TreeUnit& u, int t, int r, int start, int pos0) {
+// What the sequence's token r attends of the 32 positions from pos0 on: the context
+// from its start on, and the tokens of its mask (null: those up to its own).
+__device__ __forceinline__ uint32_t tree_visible(const TreeArgs& a, const TreeUnit& u, int r, int pos0) {
   auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; };  // bits 0 .. k - 1
   const int rel = pos0 - u.ctx;  // tree token of bit 0
-  uint32_t v = below(-rel) & ~below(start - pos0);
+  uint32_t v = below(-rel);
+  if (a.ks != nullptr && v != 0) v &= ~below(a.ks[u.q0 + r] - pos0);
   uint32_t w = 0;
   if (rel > -32 && rel < u.n) {
     if (a.mask == nullptr) {
       w = below(r + 1 - rel) & ~below(-rel);
     } else {
-      const uint64_t* row = a.mask + (int64_t)t * a.words;
+      const uint64_t* row = a.mask + (int64_t)(u.q0 + r) * a.words;
       if (rel < 0) {
         w = (uint32_t)(row[0] << -rel);
       } else {
@@ -122,10 +131,46 @@ __device__ __forceinline__ uint32_t tree_visible(const TreeArgs& a, const TreeUn
   return v | w;
 }
 
+// What a position's V brings besides its codes.
+struct TreeV {
+  float f;              // weight factor, NaN where a field is not finite
+  float mult;           // V operand: (code - mid) times this, a power of two (tiny scales: the scale)
+  uint32_t x, y;        // 32 / f and minimum / (16 f): f16 hi | 2^11 lo << 16
+};
+// w = p f LIFT stays below 2^(TAU + 6) LIFT = 2^15
+constexpr float TREE_LIFT = 32.f;
+__device__ __forceinline__ uint32_t tree_parts(float x) {
+  const uint32_t h = f32_to_f16_bits(x);
+  return h | f32_to_f16_bits((x - f16_bits_to_f32(h)) * 2048.f) << 16;
+}
+// scale sc and minimum vm (with the middle of the codes); operands of at most
+// 2^(15 - top) before the power of two.  f is in [32, 64) where the exponent allows,
+// so that the low parts of small weights are normal numbers.  A scale below f16's
+// normal numbers is the multiplier itself.
+__device__ __forceinline__ TreeV tree_v(float sc, float vm, int top) {
+  TreeV r;
+  const bool tiny = fabsf(sc) < 6.103515625e-05f, bad = !(fabsf(vm) < INFINITY) || !(fabsf(sc) < INFINITY);
+  const int e = min(max((int)((__float_as_uint(sc) >> 23) & 255u) - 132, -14), top);
+  r.mult = tiny ? sc : __uint_as_float((uint32_t)(127 + e) << 23);
+  const float f = tiny ? 1.f : sc * __uint_as_float((uint32_t)(127 - e) << 23);
+  const float inv = __builtin_amdgcn_rcpf(f);
+  r.f = bad ? __builtin_nanf("") : f * TREE_LIFT;
+  r.x = bad ? 0u : tree_parts(32.f * inv);
+  r.y = bad ? 0u : tree_parts(vm * inv * 0.0625f);
+  return r;
+}
+// row r (0 .. 3) of X at position p: its halfword
+template <int D>
+__device__ __forceinline__ uint16_t* tree_x(u32x4* xb, int p, int r) {
+  return reinterpret_cast<uint16_t*>(xb + (p >> 5) * 64 + ((p >> 2) & 3) * 16 + r) + ((p >> 4) & 1) * 4 + (p & 3);
+}
+
 // The block of 16 positions from pos on, or -1 (uniform)
 __device__ __forceinline__ int tree_page(const TreeArgs& a, const TreeUnit& u, int pos) {
+  // (a scalar load: nothing writes the table meanwhile)
+  const auto* bt = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(a.bt + (int64_t)u.b * a.max_blocks);
   const int page = pos >> a.lbs;
-  const int phys = pos < u.len && page < a.max_blocks ? a.bt[(int64_t)u.b * a.max_blocks + page] : -1;
+  const int phys = pos < u.len && page < a.max_blocks ? bt[page] : -1;
   return phys >= 0 && (int64_t)phys < a.nb ? phys : -1;
 }
 template <int TK>
@@ -150,37 +195,31 @@ struct TreeWave {
   half8 qh[CT][NS], ql[NH == 2 ? CT : 1][NH == 2 ? NS : 1];
   float qs[CT];                            // of the scores: 1, or what a query beyond f16's range was divided by
   bool qlarge;                             // some qs is not 1 (wave-uniform)
-  float m_run[CT], l_run[CT], z_run[CT];
-  floatx4 acc[CT][NB];
-  int row[CT], tok[CT], start[CT];         // query row in the sequence, its token, its first context position
-  bool live[CT];
+  float m_run[CT];
+  floatx4 acc[CT][NB], accx[CT];           // accx: lanes of row 0: the rows of X
+  int row[CT];                             // query row in the sequence, or -1
 
-  __device__ __forceinline__ void columns(const TreeArgs& a, const TreeUnit& u, int c0, int lane) {
+  // The columns, and the first and last of their first context positions over the
+  // workgroup (`none` and 0 for a wave without columns)
+  __device__ __forceinline__ void columns(const TreeArgs& a, const TreeUnit& u, int c0, int lane, int wave, int (*red)[2],
+                                          int none, int& first, int& last) {
     const int G = a.hq / a.hkv, n = lane & 15;
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const int col = c0 + 16 * ct + n;
-      live[ct] = col < u.n * G;
-      row[ct] = live[ct] ? col / G : 0;
-      tok[ct] = u.q0 + row[ct];
-      start[ct] = live[ct] && a.ks != nullptr ? max(a.ks[tok[ct]], 0) : 0;
-      m_run[ct] = MINF;
-      l_run[ct] = z_run[ct] = 0.f;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) acc[ct][b] = floatx4{0.f, 0.f, 0.f, 0.f};
-    }
-  }
-
-  // First and last of the columns' first context positions over the workgroup, `none` for a wave without columns
-  __device__ __forceinline__ void starts(int none, int lane, int wave, int (*red)[2], int& first, int& last) const {
     first = none;
     last = 0;
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
-      if (live[ct]) {
-        first = min(first, start[ct]);
-        last = max(last, start[ct]);
+    for (int ct = 0; ct < CT; ++ct) {
+      const int col = c0 + 16 * ct + n;
+      row[ct] = col < u.n * G ? col / G : -1;
+      if (row[ct] >= 0) {
+        const int start = a.ks != nullptr ? max(a.ks[u.q0 + row[ct]], 0) : 0;
+        first = min(first, start);
+        last = max(last, start);
       }
+      m_run[ct] = MINF;
+      accx[ct] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int b = 0; b < NB; ++b) acc[ct][b] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
     first = (int)wave_min_u32((uint32_t)first);
     last = (int)~wave_min_u32(~(uint32_t)last);
     if (lane == 0) {
@@ -188,10 +227,8 @@ struct TreeWave {
       red[wave][1] = last;
     }
     __syncthreads();
-    first = min(min(red[0][0], red[1][0]), min(red[2][0], red[3][0]));
-    last = max(max(red[0][1], red[1][1]), max(red[2][1], red[3][1]));
-    first = __builtin_amdgcn_readfirstlane(first);
-    last = __builtin_amdgcn_readfirstlane(last);
+    first = __builtin_amdgcn_readfirstlane(min(min(red[0][0], red[1][0]), min(red[2][0], red[3][0])));
+    last = __builtin_amdgcn_readfirstlane(max(max(red[0][1], red[1][1]), max(red[2][1], red[3][1])));
   }
 
   // The columns' queries, rotated and scaled, as f16 hi + lo.  One query per 16
@@ -200,7 +237,7 @@ struct TreeWave {
     constexpr int E = D / 16;
     const int G = a.hq / a.hkv, l16 = lane & 15, g = lane >> 4, n = lane & 15;
     qlarge = false;
-#pragma unroll 1
+#pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       float inv = 1.f;
 #pragma unroll 1
@@ -244,7 +281,6 @@ struct TreeWave {
         for (int i = 0; i < E; ++i) rows[4 * k + g][l16 * E + i] = y[i] * up;
       }
       __asm__ volatile("" ::: "memory");  // a wave's LDS accesses run in order
-      half8 hi[NS], lo[NS];
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         uint32_t h[4], l[4];
@@ -254,30 +290,21 @@ struct TreeWave {
           h[j] = pk_f16(x, y);
           l[j] = NH == 2 ? pk_f16(f16_rest(x, h[j], 0), f16_rest(y, h[j], 1)) : 0u;
         }
-        hi[s] = __builtin_bit_cast(half8, u32x4{h[0], h[1], h[2], h[3]});
-        lo[s] = __builtin_bit_cast(half8, u32x4{l[0], l[1], l[2], l[3]});
+        qh[ct][s] = __builtin_bit_cast(half8, u32x4{h[0], h[1], h[2], h[3]});
+        if constexpr (NH == 2) ql[ct][s] = __builtin_bit_cast(half8, u32x4{l[0], l[1], l[2], l[3]});
       }
       __asm__ volatile("" ::: "memory");
-#pragma unroll
-      for (int c = 0; c < CT; ++c)
-        if (c == ct) {  // (register arrays need constant indexes)
-          qs[c] = inv;
-#pragma unroll
-          for (int s = 0; s < NS; ++s) {
-            qh[c][s] = hi[s];
-            if constexpr (NH == 2) ql[c][s] = lo[s];
-          }
-        }
+      qs[ct] = inv;
       qlarge = qlarge || __builtin_amdgcn_ballot_w64(inv != 1.f) != 0;
     }
   }
 
-  // One tile of the positions from pos0 on: kb, vb its operands ([k][part][NS] and
-  // [p][part][NB] units of 64), tb its factors.  edge (uniform): some column does not
-  // attend all of it, or (bit k of `on`: positions 16 k .. have a page) nobody some.
-  // next(): called behind the reads of the K operands.
+  // One tile of the positions from pos0 on: kb, vb, xb its operands ([k][part][NS],
+  // [p][part][NB] and [p] units of 64), tb its factors.  edge (uniform): some column
+  // does not attend all of it, or (bit k of `on`: positions 16 k .. have a page) nobody
+  // some.  next(): called behind the score products.
   template <typename F>
-  __device__ __forceinline__ void tile(const TreeArgs& a, const TreeUnit& u, const u32x4* kb, const u32x4* vb,
+  __device__ __forceinline__ void tile(const TreeArgs& a, const TreeUnit& u, const u32x4* kb, const u32x4* vb, const u32x4* xb,
                                        const float (*tb)[TK], int pos0, bool edge, uint32_t on, int lane, F next) {
     const int g = lane >> 4;
     floatx4 s[NT][CT];
@@ -285,43 +312,48 @@ struct TreeWave {
     for (int k = 0; k < NT; ++k)
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) s[k][ct] = floatx4{0.f, 0.f, 0.f, 0.f};
+    constexpr int AHEAD = KHL ? 1 : NS;  // steps whose K operands are requested together
 #pragma unroll
-    for (int d = 0; d < NS; ++d) {
-      half8 xh[NT], xl[NT];
+    for (int d0 = 0; d0 < NS; d0 += AHEAD) {
+      half8 xh[AHEAD][NT], xl[AHEAD][NT];
+#pragma unroll
+      for (int d = 0; d < AHEAD; ++d)
+#pragma unroll
+        for (int k = 0; k < NT; ++k) {
+          const int at = C::kunit(d0 + d, lane & 15, g);
+          xh[d][k] = __builtin_bit_cast(half8, kb[(k * KP) * NS * 64 + at]);
+          if constexpr (KHL) xl[d][k] = __builtin_bit_cast(half8, kb[(k * KP + 1) * NS * 64 + at]);
+        }
+      if constexpr (!KHL) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < AHEAD; ++d) {
+        // the low products first: what they add is not lost beside the high ones' sum
+        if constexpr (NH == 2) {
+#pragma unroll
+          for (int k = 0; k < NT; ++k)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[d][k], ql[ct][d0 + d], s[k][ct], 0, 0, 0);
+        }
+        if constexpr (KHL) {
+#pragma unroll
+          for (int k = 0; k < NT; ++k)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl[d][k], qh[ct][d0 + d], s[k][ct], 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < NT; ++k)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[d][k], qh[ct][d0 + d], s[k][ct], 0, 0, 0);
+      }
+    }
+    next();
+    float tf[2][NT][4];  // the factors of this lane's positions 16 k + 4 g + i
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
 #pragma unroll
       for (int k = 0; k < NT; ++k) {
-        const int at = C::kunit(d, lane & 15, g);
-        xh[k] = __builtin_bit_cast(half8, kb[(k * KP) * NS * 64 + at]);
-        if constexpr (KHL) xl[k] = __builtin_bit_cast(half8, kb[(k * KP + 1) * NS * 64 + at]);
-      }
-      // the low products first: what they add is not lost beside the high ones' sum
-      if constexpr (NH == 2) {
-#pragma unroll
-        for (int k = 0; k < NT; ++k)
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[k], ql[ct][d], s[k][ct], 0, 0, 0);
-      }
-      if constexpr (KHL) {
-#pragma unroll
-        for (int k = 0; k < NT; ++k)
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl[k], qh[ct][d], s[k][ct], 0, 0, 0);
-      }
-#pragma unroll
-      for (int k = 0; k < NT; ++k)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[k], qh[ct][d], s[k][ct], 0, 0, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);  // the next tile's operands are not formed beside this one's reads (registers)
-    next();
-    __builtin_amdgcn_sched_barrier(0);
-    float tf[NT][3][4];  // the factors of this lane's positions 16 k + 4 g + i
-#pragma unroll
-    for (int k = 0; k < NT; ++k)
-#pragma unroll
-      for (int f = 0; f < 3; ++f) {
         const float4 x = *reinterpret_cast<const float4*>(&tb[f][16 * k + 4 * g]);
-        tf[k][f][0] = x.x; tf[k][f][1] = x.y; tf[k][f][2] = x.z; tf[k][f][3] = x.w;
+        tf[f][k][0] = x.x; tf[f][k][1] = x.y; tf[f][k][2] = x.z; tf[f][k][3] = x.w;
       }
     if (qlarge) {
 #pragma unroll
@@ -329,62 +361,70 @@ struct TreeWave {
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) s[k][ct] *= qs[ct];
     }
+    floatx4 y[NT][CT];  // scores less the running maximum
 #pragma unroll
     for (int k = 0; k < NT; ++k)
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[k][ct][i] *= tf[k][0][i];
+        for (int i = 0; i < 4; ++i) y[k][ct][i] = __builtin_fmaf(s[k][ct][i], tf[0][k][i], -m_run[ct]);
     if (edge) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
           const uint32_t held = ((on >> (2 * p)) & 1u ? 0xffffu : 0u) | ((on >> (2 * p + 1)) & 1u ? 0xffff0000u : 0u);
-          uint32_t vis = live[ct] ? tree_visible(a, u, tok[ct], row[ct], start[ct], pos0 + 32 * p) & held : 0u;
+          uint32_t vis = row[ct] >= 0 ? tree_visible(a, u, row[ct], pos0 + 32 * p) & held : 0u;
           vis >>= 4 * g;
 #pragma unroll
           for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (((vis >> (16 * k + i)) & 1u) == 0) s[2 * p + k][ct][i] = -INFINITY;
+              if (((vis >> (16 * k + i)) & 1u) == 0) y[2 * p + k][ct][i] = -INFINITY;
         }
     }
+    float tm = y[0][0][0];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      float tm = s[0][ct][0];
+    for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
       for (int k = 0; k < NT; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tm = fmaxf(tm, s[k][ct][i]);
-      tm = warp_max_q(tm);
-      if (__builtin_amdgcn_ballot_w64(tm > m_run[ct] + TAU) != 0) {  // wave-uniform, rare
-        const float mn = fmaxf(m_run[ct], tm);
+        for (int i = 0; i < 4; ++i) tm = fmaxf(tm, y[k][ct][i]);
+    if (__builtin_amdgcn_ballot_w64(tm > TAU) != 0) {  // wave-uniform, rare: raise the maxima
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < NT; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            y[k][ct][i] = y[k][ct][i] == -INFINITY ? -INFINITY : s[k][ct][i] * tf[0][k][i];
+            mx = fmaxf(mx, y[k][ct][i]);
+          }
+        const float mn = fmaxf(m_run[ct], warp_max_q(mx));
         const float al = __builtin_amdgcn_exp2f(m_run[ct] - mn);
         m_run[ct] = mn;
-        l_run[ct] *= al;
-        z_run[ct] *= al;
+#pragma unroll
+        for (int k = 0; k < NT; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[k][ct][i] -= mn;
+        accx[ct] *= al;
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[ct][b] *= al;
       }
     }
-    // weights: p; p x V minimum kept aside; p x V factor as f16 parts.  A tile's
-    // sums are formed first, so that many small weights beside a large one count.
+    // weights x V factor as f16 parts
     u32x4 ph[NP][CT], pl[NH == 2 ? NP : 1][NH == 2 ? CT : 1];
     auto weights = [&](auto masked) __attribute__((always_inline)) {
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        float lt = 0.f, zt = 0.f;
+      for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
         for (int k = 0; k < NT; ++k) {
           float w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const bool hid = decltype(masked)::value && s[k][ct][i] == -INFINITY;  // its factors may be infinite or NaN
-            const float e = __builtin_amdgcn_exp2f(s[k][ct][i] - m_run[ct]);
-            lt += e;
-            zt = __builtin_fmaf(e, hid ? 0.f : tf[k][2][i], zt);
-            w[i] = e * (hid ? 0.f : tf[k][1][i]);
+            const bool hid = decltype(masked)::value && y[k][ct][i] == -INFINITY;  // its factor may be NaN
+            w[i] = __builtin_amdgcn_exp2f(y[k][ct][i]) * (hid ? 0.f : tf[1][k][i]);
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -393,53 +433,55 @@ struct TreeWave {
             if constexpr (NH == 2) pl[k >> 1][ct][2 * (k & 1) + h] = pk_f16(f16_rest(w[2 * h], hi, 0), f16_rest(w[2 * h + 1], hi, 1));
           }
         }
-        l_run[ct] += lt;
-        z_run[ct] += zt;
-      }
     };
     if (edge) weights(std::true_type{});
     else weights(std::false_type{});
-    auto of = [](const u32x4& w, int b) { return __builtin_bit_cast(half8, C::vx(b) ? u32x4{w[2], w[3], w[0], w[1]} : w); };
+    auto of = [](const u32x4& w, bool swap) { return __builtin_bit_cast(half8, swap ? u32x4{w[2], w[3], w[0], w[1]} : w); };
+    auto product = [&](half8 x, floatx4& c, int p, int ct, bool swap) __attribute__((always_inline)) {
+      if constexpr (NH == 2) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, of(pl[p][ct], swap), c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, of(ph[p][ct], swap), c, 0, 0, 0);
+    };
 #pragma unroll
-    for (int p = 0; p < NP; ++p)
+    for (int p = 0; p < NP; ++p) {
+      const half8 x = __builtin_bit_cast(half8, xb[p * 64 + lane]);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) product(x, accx[ct], p, ct, false);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const half8 x = __builtin_bit_cast(half8, vb[(p * VP * NB + b) * 64 + lane]);
+        const half8 v = __builtin_bit_cast(half8, vb[(p * VP * NB + b) * 64 + lane]);
         if constexpr (VHL) {
-          const half8 y = __builtin_bit_cast(half8, vb[((p * VP + 1) * NB + b) * 64 + lane]);
+          const half8 lo = __builtin_bit_cast(half8, vb[((p * VP + 1) * NB + b) * 64 + lane]);
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, of(ph[p][ct], b), acc[ct][b], 0, 0, 0);
-        }
-        if constexpr (NH == 2) {
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, of(pl[p][ct], b), acc[ct][b], 0, 0, 0);
+          for (int ct = 0; ct < CT; ++ct) acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, of(ph[p][ct], C::vx(b)), acc[ct][b], 0, 0, 0);
         }
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, of(ph[p][ct], b), acc[ct][b], 0, 0, 0);
+        for (int ct = 0; ct < CT; ++ct) product(v, acc[ct][b], p, ct, C::vx(b));
       }
+    }
   }
 
-  // Lane (n, g) holds dims NB (4 g + i) + b of column n.  vscale undoes the common
-  // power of two of the weights' factors.
-  __device__ __forceinline__ void finish(const TreeArgs& a, const TreeUnit& u, int c0, int lane, float vscale) {
+  // Lane (n, g) holds dims NB (4 g + i) + b of column n.
+  __device__ __forceinline__ void finish(const TreeArgs& a, const TreeUnit& u, int c0, int lane) {
     const int n = lane & 15, g = lane >> 4, G = a.hq / a.hkv;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const float L = warp_sum_q(l_run[ct]), Z = warp_sum_q(z_run[ct]);
+      // sums of the weights and of the minima, both times LIFT, from the lanes g = 0
+      const float L = __shfl(__builtin_fmaf(accx[ct][1], 1.f / 2048.f, accx[ct][0]), n) * (1.f / 32.f);
+      const float Z = __shfl(__builtin_fmaf(accx[ct][3], 1.f / 2048.f, accx[ct][2]), n) * 16.f;
       const bool none = L == 0.f;  // no position; a NaN score makes L, and the output, NaN
       const float inv = none ? 0.f : 1.f / L;
       float y[4][NB];
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i][b] = none ? 0.f : __builtin_fmaf(acc[ct][b][i], vscale, Z) * inv;
-      const int64_t at = (int64_t)tok[ct] * a.hq + u.kvh * G + (c0 + 16 * ct + n - row[ct] * G);
+        for (int i = 0; i < 4; ++i) y[i][b] = none ? 0.f : (acc[ct][b][i] + Z) * inv;
+      const int64_t at = (int64_t)(u.q0 + row[ct]) * a.hq + u.kvh * G + (c0 + 16 * ct + n - row[ct] * G);
       if (a.wo != nullptr) {
-        if (live[ct]) {
+        if (row[ct] >= 0) {
           const int64_t r = at * a.splits + u.split;
 #pragma unroll
           for (int i = 0; i < 4; ++i) store_elems<F32, NB>(a.wo, r * D + NB * (4 * g + i), y[i]);
-          if (g == 0) a.wl[r] = none ? -INFINITY : m_run[ct] + __builtin_log2f(L);
+          if (g == 0) a.wl[r] = none ? -INFINITY : m_run[ct] + __builtin_log2f(L * (1.f / TREE_LIFT));
         }
         continue;
       }
@@ -463,7 +505,7 @@ struct TreeWave {
           for (int i = 0; i < 4; ++i) y[i][b] = fwht_pair32(fwht_pair16(y[i][b], g & 1), g & 2) * a.oscale;
         }
       }
-      if (live[ct]) {
+      if (row[ct] >= 0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int64_t off = at * D + NB * (4 * g + i);
@@ -471,7 +513,7 @@ struct TreeWave {
           else if (a.ot == F16) store_elems<F16, NB>(a.out, off, y[i]);
           else store_elems<BF16, NB>(a.out, off, y[i]);
         }
-        if (a.lse != nullptr && g == 0) a.lse[at] = none ? -INFINITY : (m_run[ct] + __builtin_log2f(L)) * 0.69314718055994531f;
+        if (a.lse != nullptr && g == 0) a.lse[at] = none ? -INFINITY : (m_run[ct] + __builtin_log2f(L * (1.f / TREE_LIFT))) * 0.69314718055994531f;
       }
     }
   }

@@ -145,21 +145,24 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
           // factor, so that the rows that attend it are NaN and the others, whose
           // products meet it with a weight of 0, are not.
           float fk = 1.f;
-          TreeV v{beyond == 0.f ? TREE_LIFT : __builtin_nanf(""), beyond == 0.f ? 1.f : 0.f, beyond == 0.f ? tree_parts(32.f) : 0u, 0u};
+          TreeV v{beyond == 0.f ? TREE_LIFT : __builtin_nanf(""), beyond == 0.f ? 1.f : 0.f, beyond == 0.f ? 0x5000u : 0u, 0u};
           if (!raw) {
             if (!kf8) fk = f16_bits_to_f32(row_bits(row, 8 * geo.mse, 16)) / __builtin_sqrtf(csq + 1e-16f) * table_scale_inv;
             float sc = f16_bits_to_f32(row_bits(row, 8 * (geo.kps + geo.vdb), 16)), vm = 0.f;
-            if constexpr (LM) sc = sc / __builtin_sqrtf(vsq + 1e-16f) * (512.f * table_scale_inv);  // the norm's
+            if constexpr (LM) {  // the norm's; a minimum of 0, or NaN where the norm is not finite
+              sc = sc / __builtin_sqrtf(vsq + 1e-16f) * (512.f * table_scale_inv);
+              vm = sc * 0.f;
+            }
             else vm = __builtin_fmaf(mid, sc, f16_bits_to_f32(row_bits(row, 8 * (geo.kps + geo.vdb) + 16, 16)));
             // (codes of 128 at most times 2^8; Lloyd-Max values are below 2)
             v = tree_v(sc, vm, LM ? 14 : a.vb == 8 ? 8 : 11);
           }
           tb[0][p] = fk;
           tb[1][p] = v.f;
-          *tree_x<D>(xb, p, 0) = (uint16_t)v.x;
-          *tree_x<D>(xb, p, 1) = (uint16_t)(v.x >> 16);
-          *tree_x<D>(xb, p, 2) = (uint16_t)v.y;
-          *tree_x<D>(xb, p, 3) = (uint16_t)(v.y >> 16);
+          *tree_x<D>(xb, p, 0) = (uint16_t)v.hi;
+          *tree_x<D>(xb, p, 1) = (uint16_t)(v.hi >> 16);
+          *tree_x<D>(xb, p, 2) = (uint16_t)v.lo;
+          *tree_x<D>(xb, p, 3) = (uint16_t)(v.lo >> 16);
           vex[p] = v.mult;
         }
       }
@@ -213,7 +216,7 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
       }
       __syncthreads();
       const uint32_t on = tree_held<TK>(a, u, pos0);  // bit k: positions 16 k .. of the tile have a page
-      w.tile(a, u, kf, vf, xb, tb, pos0, pos0 < last || pos0 + TK > u.ctx || on != (1u << NT) - 1u, on, lane, [] {});
+      w.tile(a, u, kf, vf, xb, tb, pos0, pos0 < last || pos0 + TK > u.ctx || on != (1u << NT) - 1u, on, lane, [](auto) {});
       __syncthreads();  // before the next tile's rows
     }
     w.finish(a, u, c0, lane);

@@ -25,23 +25,17 @@ namespace ftq {
 struct __attribute__((packed, aligned(2))) TreeU32 { uint32_t v; };
 struct __attribute__((packed, aligned(2))) TreeU64 { uint64_t v; };
 
-// Bytes that one lane reads of one position's codes, from an even offset
+// N bytes (a multiple of 4) from an even offset
 template <int N>
-__device__ __forceinline__ void tree_bytes(const uint8_t* p, uint32_t (&w)[(N + 3) / 4]) {
-  if constexpr (N == 1) {
-    w[0] = *p;
-  } else if constexpr (N == 2) {
-    w[0] = *reinterpret_cast<const uint16_t*>(p);
-  } else {
+__device__ __forceinline__ void tree_bytes(const uint8_t* p, uint32_t (&w)[N / 4]) {
 #pragma unroll
-    for (int i = 0; i < (N + 3) / 4; i += 2) {
-      if (N - 4 * i > 4) {  // 6 bytes read 8: the slot goes on behind its codes
-        const uint64_t x = reinterpret_cast<const TreeU64*>(p + 4 * i)->v;
-        w[i] = (uint32_t)x;
-        w[i + 1] = (uint32_t)(x >> 32);
-      } else {
-        w[i] = reinterpret_cast<const TreeU32*>(p + 4 * i)->v;
-      }
+  for (int i = 0; i < N / 4; i += 2) {
+    if (i + 1 < N / 4) {
+      const uint64_t x = reinterpret_cast<const TreeU64*>(p + 4 * i)->v;
+      w[i] = (uint32_t)x;
+      w[i + 1] = (uint32_t)(x >> 32);
+    } else {
+      w[i] = reinterpret_cast<const TreeU32*>(p + 4 * i)->v;
     }
   }
 }
@@ -64,55 +58,59 @@ struct TreeFmt {
   static constexpr int TPW = C::TK / 4;                     // positions of a wave
   static constexpr int LPT = 64 / TPW, EK = D / LPT;        // K: lanes of a position, dims of a lane
   static constexpr int LPQ = 256 / TPW, DV = D / LPQ;       // V: lanes of four positions, dims of a lane
-  static constexpr int KN = EK * KB / 8;                    // bytes of a lane's K codes
-  static constexpr int VBITS = DV * VB;
-  static constexpr bool VSH = VBITS % 16 != 0 && VBITS != 8;  // V codes that start inside a 16-bit unit
-  static constexpr int VN = VBITS == 8 ? 1 : VSH ? 4 : VBITS / 8;
+  // Loads are whole dwords from even offsets (16-bit ones would be converted, and
+  // waited for, as they come); what they read past a lane's codes lies in the slot.
+  static constexpr int KN = EK * KB / 8, KR = (KN + 3) / 4 * 4;  // bytes of a lane's K codes, and read
+  static constexpr int VBITS = DV * VB;                     // a lane's V codes of one position
+  static constexpr bool VSH = VBITS % 16 != 0;              // ... that may start inside a 16-bit unit
+  static constexpr int VR = RAW ? VBITS / 8 : 4;            // bytes read for them
   static constexpr int ENTRIES = RAW ? 1 : 1 << (2 * KB);
   static constexpr float MID = 0.5f * (float)((1 << (RAW ? 0 : VB)) - 1);
 
-  uint32_t k[(KN + 3) / 4], v[4][(VN + 3) / 4];
+  uint32_t k[KR / 4], v[4][VR / 4];
   uint32_t kn, sm;  // K norm of the lane's position; scale | minimum of V position lane % 4 of its four
 
   // base: slot of the wave's first position (uniform)
   __device__ __forceinline__ void load(const uint8_t* base, uint32_t s_pos, int lane) {
     const int e = lane % LPT, dq = lane % LPQ;
-    const uint32_t ko = (uint32_t)(lane / LPT) * s_pos, vo = (uint32_t)(lane / LPQ * 4) * s_pos;
-    const uint32_t off = vo + (uint32_t)G.kps + (VBITS == 8 ? dq : (uint32_t)(dq * VBITS) >> 4 << 1);
+    uint32_t kn_at = (uint32_t)(lane / LPT) * s_pos, k_at = kn_at + e * KN;
+    uint32_t v_at = (uint32_t)(lane / LPQ * 4) * s_pos, sm_at = v_at + (uint32_t)(dq & 3) * s_pos;
+    v_at += (uint32_t)(dq * VBITS) >> 4 << 1;
+    // (opaque here, so that each stays the 32-bit offset of a uniform address)
+    __asm__ volatile("" : "+v"(kn_at), "+v"(k_at), "+v"(v_at), "+v"(sm_at));
     if constexpr (RAW) {
 #pragma unroll
       for (int i = 0; i < KN / 16; ++i) {
-        const uint4 x = *reinterpret_cast<const uint4*>(base + (ko + e * KN) + 16 * i);
+        const uint4 x = *reinterpret_cast<const uint4*>(base + k_at + 16 * i);
         k[4 * i] = x.x; k[4 * i + 1] = x.y; k[4 * i + 2] = x.z; k[4 * i + 3] = x.w;
       }
     } else {
-      tree_bytes<KN>(base + (ko + e * KN), k);
-      kn = *reinterpret_cast<const uint16_t*>(base + ko + G.mse);
+      tree_bytes<KR>(base + k_at, k);
+      kn = reinterpret_cast<const TreeU32*>(base + kn_at + G.mse)->v;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint8_t* pv = base + (int64_t)i * s_pos;  // uniform
+      uint64_t row = (uint64_t)i * s_pos + G.kps;
+      __asm__("" : "+s"(row));  // uniform, and added to the base first
+      const uint8_t* pv = base + row;
       if constexpr (RAW) {
-        if constexpr (VN == 8) {
-          const uint2 x = *reinterpret_cast<const uint2*>(pv + off);
+        if constexpr (VR == 8) {
+          const uint2 x = *reinterpret_cast<const uint2*>(pv + v_at);
           v[i][0] = x.x; v[i][1] = x.y;
         } else {
-          const uint4 x = *reinterpret_cast<const uint4*>(pv + off);
+          const uint4 x = *reinterpret_cast<const uint4*>(pv + v_at);
           v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
         }
       } else {
-        tree_bytes<VN>(pv + off, v[i]);
+        tree_bytes<VR>(pv + v_at, v[i]);
       }
     }
-    if constexpr (!RAW) sm = reinterpret_cast<const TreeU32*>(base + (vo + (uint32_t)(dq & 3) * s_pos) + (G.kps + G.vdb))->v;
+    if constexpr (!RAW) sm = reinterpret_cast<const TreeU32*>(base + sm_at + (G.kps + G.vdb))->v;
   }
 
-  // To operands of the tile's positions TPW w .., in a buffer
-  __device__ __forceinline__ void emit(const uint32_t* table, u32x4* buf, int w, int lane) const {
-    using B = TreeBuf<D>;
-    u32x4 *kb = buf, *vb = buf + B::V, *xb = buf + B::X;
-    float(*tb)[C::TK] = reinterpret_cast<float(*)[C::TK]>(buf + B::T);
-    constexpr int NS = C::NS, NB = C::NB;
+  // K operands and factors of the tile's positions TPW w .., to a buffer
+  __device__ __forceinline__ void emit_k(const uint32_t* table, u32x4* buf, int w, int lane) const {
+    constexpr int NS = C::NS;
     const int p = w * TPW + lane / LPT, e = lane % LPT, d0 = e * EK;
     float csq = 0.f;
 #pragma unroll
@@ -129,14 +127,19 @@ struct TreeFmt {
         }
       }
       const int d = d0 + 8 * u;
-      kb[(p >> 4) * NS * 64 + C::kunit(d / 32, p & 15, (d / 8) & 3)] = x;
+      buf[(p >> 4) * NS * 64 + C::kunit(d / 32, p & 15, (d / 8) & 3)] = x;
     }
-    if constexpr (!RAW) {
-      csq = group_sum<LPT>(csq);
-      if (e == 0) tb[0][p] = f16_bits_to_f32(kn) * __builtin_amdgcn_rsqf(csq + 1e-16f);
-    } else if (e == 0) {
-      tb[0][p] = 1.f;
-    }
+    // the lanes of a position all have its factor, and write it to one place
+    float* tb = reinterpret_cast<float*>(buf + TreeBuf<D>::T);
+    if constexpr (!RAW) tb[p] = f16_bits_to_f32(kn & 0xffffu) * __builtin_amdgcn_rsqf(group_sum<LPT>(csq) + 1e-16f);
+    else tb[p] = 1.f;
+  }
+
+  // V and X operands and factors
+  __device__ __forceinline__ void emit_v(u32x4* buf, int w, int lane) const {
+    constexpr int NB = C::NB;
+    u32x4 *vb = buf + TreeBuf<D>::V, *xb = buf + TreeBuf<D>::X;
+    float* tb = reinterpret_cast<float*>(buf + TreeBuf<D>::T) + C::TK;
     // V: positions 4 q ..
     const int q = w * (TPW / 4) + lane / LPQ, dq = lane % LPQ;
     uint2* out = reinterpret_cast<uint2*>(vb + (q >> 3) * NB * 64 + (q & 3) * 16);
@@ -165,23 +168,21 @@ struct TreeFmt {
         hi &= (bad & 4 ? 0u : 0xffffu) | (bad & 8 ? 0u : 0xffff0000u);
         put(i, lo, hi);
       }
-      if (dq < 4) {
-        const bool b = (bad >> dq) & 1;
-        tb[1][4 * q + dq] = b ? __builtin_nanf("") : TREE_LIFT;
-        *tree_x<D>(xb, 4 * q + dq, 0) = b ? 0 : 0x5000;  // 32
-      }
+      const int own = dq & 3;  // lanes with the same write the same
+      const bool b = (bad >> own) & 1;
+      tb[4 * q + own] = b ? __builtin_nanf("") : TREE_LIFT;
+      *tree_x<D>(xb, 4 * q + own, 0) = b ? 0 : 0x5000;  // 32
     } else {
       // the lane's own position; operand (code - mid) mult = (1 + code 2^-VB) 2^VB mult
       // - (2^VB + mid) mult
       const float sc = f16_bits_to_f32(sm & 0xffffu);
       const TreeV r = tree_v(sc, __builtin_fmaf(MID, sc, f16_bits_to_f32(sm >> 16)), 11);
-      if (dq < 4) {
-        tb[1][4 * q + dq] = r.f;
-        *tree_x<D>(xb, 4 * q + dq, 0) = (uint16_t)r.x;
-        *tree_x<D>(xb, 4 * q + dq, 1) = (uint16_t)(r.x >> 16);
-        *tree_x<D>(xb, 4 * q + dq, 2) = (uint16_t)r.y;
-        *tree_x<D>(xb, 4 * q + dq, 3) = (uint16_t)(r.y >> 16);
-      }
+      const int own_p = 4 * q + (dq & 3);  // lanes with the same write the same
+      tb[own_p] = r.f;
+      *tree_x<D>(xb, own_p, 0) = (uint16_t)r.hi;
+      *tree_x<D>(xb, own_p, 1) = (uint16_t)(r.hi >> 16);
+      *tree_x<D>(xb, own_p, 2) = (uint16_t)r.lo;
+      *tree_x<D>(xb, own_p, 3) = (uint16_t)(r.lo >> 16);
       const uint32_t own = pk_f16(r.mult * (float)(1 << VB), r.mult * -((float)(1 << VB) + MID));
       uint32_t ec[4];  // of the four positions: from the four lanes of a quad
       ec[0] = (uint32_t)__builtin_amdgcn_mov_dpp((int)own, 0x00, 0xF, 0xF, true);
@@ -280,39 +281,41 @@ __global__ __launch_bounds__(256, 2) void tree_fast_kernel(const TreeArgs a) {
     uint32_t on = 0;  // runs of 16 with a page, of the tile in `raw`
     const int32_t* bt = a.bt + (int64_t)u.b * a.max_blocks;
     auto entries = [&](int t) __attribute__((always_inline)) {
-      const int pos = t * TK + 16 * (lane & (NT - 1)), at = pos >> a.lbs;
-      entry = pos < u.len && at < a.max_blocks ? bt[at] : -1;
+      entry = bt[min((t * TK + 16 * (lane & (NT - 1))) >> a.lbs, a.max_blocks - 1)];
     };
     auto fetch = [&](int t) __attribute__((always_inline)) {  // tile t's bytes, and the next one's entries
-      const bool ok = (uint32_t)entry < (uint32_t)nb32;
+      const int pos = t * TK + 16 * (lane & (NT - 1));
+      const bool ok = pos < held && (uint32_t)entry < (uint32_t)nb32;
       on = (uint32_t)__builtin_amdgcn_ballot_w64(ok) & ((1u << NT) - 1u);
       const int page = __builtin_amdgcn_readlane(ok ? entry : 0, sub);  // positions without one read block 0
       const int64_t at = (int64_t)page * a.sblk + (int64_t)((t * TK + 16 * sub) & ((1 << a.lbs) - 1)) * a.spos;
       raw.load(head + at, s_pos, lane);
-      entries(t + 1);
+      entries(min(t + 1, tb1 - 1));
     };
-    uint32_t on_now = 0;
+    uint32_t now = 0;  // `on` of the tile that is multiplied
     if (tb0 < tb1) {
       entries(tb0);
       fetch(tb0);
-      raw.emit(table, pool, wave, lane);
-      on_now = on;
-      if (tb0 + 1 < tb1) fetch(tb0 + 1);
+      raw.emit_k(table, pool, wave, lane);
+      raw.emit_v(pool, wave, lane);
+      now = on;
+      fetch(min(tb0 + 1, tb1 - 1));
     }
     int p = 0;
     for (int t = tb0; t < tb1; ++t, p ^= 1) {
       tree_barrier();
       const int pos0 = t * TK;
       const u32x4* buf = pool + p * B::SIZE;
-      const uint32_t now = on_now;
-      auto next = [&]() __attribute__((always_inline)) {
-        if (t + 1 < tb1) {
-          raw.emit(table, pool + (p ^ 1) * B::SIZE, wave, lane);
-          on_now = on;
-          if (t + 2 < tb1) fetch(t + 2);
-        }
+      u32x4* to = pool + (p ^ 1) * B::SIZE;
+      // (behind the last tile: it again, for nobody)
+      auto beside = [&](auto part) __attribute__((always_inline)) {
+        if constexpr (decltype(part)::value == 0) raw.emit_k(table, to, wave, lane);
+        else raw.emit_v(to, wave, lane);
       };
-      w.tile(a, u, buf, buf + B::V, buf + B::X, reinterpret_cast<const float(*)[TK]>(buf + B::T), pos0, pos0 < last || pos0 + TK > u.ctx || now != (1u << NT) - 1u, now, lane, next);
+      w.tile(a, u, buf, buf + B::V, buf + B::X, reinterpret_cast<const float(*)[TK]>(buf + B::T), pos0,
+             pos0 < last || pos0 + TK > u.ctx || now != (1u << NT) - 1u, now, lane, beside);
+      now = on;
+      fetch(min(t + 2, tb1 - 1));
     }
     w.finish(a, u, c0, lane);
   }

@@ -135,31 +135,38 @@ __device__ __forceinline__ uint32_t tree_visible(const TreeArgs& a, const TreeUn
 struct TreeV {
   float f;              // weight factor, NaN where a field is not finite
   float mult;           // V operand: (code - mid) times this, a power of two (tiny scales: the scale)
-  uint32_t x, y;        // 32 / f and minimum / (16 f): f16 hi | 2^11 lo << 16
+  uint32_t hi, lo;      // 32 / f and minimum / (16 f): f16 parts (x | y << 16), the low ones times 2^11
 };
 // w = p f LIFT stays below 2^(TAU + 6) LIFT = 2^15
 constexpr float TREE_LIFT = 32.f;
-__device__ __forceinline__ uint32_t tree_parts(float x) {
-  const uint32_t h = f32_to_f16_bits(x);
-  return h | f32_to_f16_bits((x - f16_bits_to_f32(h)) * 2048.f) << 16;
+// f16 parts of x and y
+__device__ __forceinline__ void tree_parts(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pk_f16(x, y);
+  lo = pk_f16(f16_rest(x, hi, 0) * 2048.f, f16_rest(y, hi, 1) * 2048.f);
 }
-// scale sc and minimum vm (with the middle of the codes); operands of at most
-// 2^(15 - top) before the power of two.  f is in [32, 64) where the exponent allows,
-// so that the low parts of small weights are normal numbers.  A scale below f16's
-// normal numbers is the multiplier itself.
+// scale sc and minimum vm (with the middle of the codes times sc: not finite where
+// either is not); operands of at most 2^(15 - top) before the power of two.  f is in
+// [32, 64) where the exponent allows, so that the low parts of small weights are
+// normal numbers.  A scale below f16's normal numbers is the multiplier itself.
 __device__ __forceinline__ TreeV tree_v(float sc, float vm, int top) {
   TreeV r;
-  const bool tiny = fabsf(sc) < 6.103515625e-05f, bad = !(fabsf(vm) < INFINITY) || !(fabsf(sc) < INFINITY);
+  const bool tiny = fabsf(sc) < 6.103515625e-05f, bad = !(fabsf(vm) < INFINITY);
   const int e = min(max((int)((__float_as_uint(sc) >> 23) & 255u) - 132, -14), top);
   r.mult = tiny ? sc : __uint_as_float((uint32_t)(127 + e) << 23);
   const float f = tiny ? 1.f : sc * __uint_as_float((uint32_t)(127 - e) << 23);
   const float inv = __builtin_amdgcn_rcpf(f);
+  tree_parts(32.f * inv, vm * inv * 0.0625f, r.hi, r.lo);
   r.f = bad ? __builtin_nanf("") : f * TREE_LIFT;
-  r.x = bad ? 0u : tree_parts(32.f * inv);
-  r.y = bad ? 0u : tree_parts(vm * inv * 0.0625f);
+  r.hi = bad ? 0u : r.hi;
+  r.lo = bad ? 0u : r.lo;
   return r;
 }
-// row r (0 .. 3) of X at position p: its halfword
+__device__ __forceinline__ float tree_max3(float a, float b, float c) {
+  float r;  // (fmaxf would quiet each operand first)
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// row r (0 .. 3: x high, y high, x low, y low) of X at position p: its halfword
 template <int D>
 __device__ __forceinline__ uint16_t* tree_x(u32x4* xb, int p, int r) {
   return reinterpret_cast<uint16_t*>(xb + (p >> 5) * 64 + ((p >> 2) & 3) * 16 + r) + ((p >> 4) & 1) * 4 + (p & 3);
@@ -194,7 +201,7 @@ struct TreeWave {
 
   half8 qh[CT][NS], ql[NH == 2 ? CT : 1][NH == 2 ? NS : 1];
   float qs[CT];                            // of the scores: 1, or what a query beyond f16's range was divided by
-  bool qlarge;                             // some qs is not 1 (wave-uniform)
+  int qlarge;                              // some qs is not 1 (wave-uniform)
   float m_run[CT];
   floatx4 acc[CT][NB], accx[CT];           // accx: lanes of row 0: the rows of X
   int row[CT];                             // query row in the sequence, or -1
@@ -236,7 +243,7 @@ struct TreeWave {
   __device__ __forceinline__ void queries(const TreeArgs& a, const TreeUnit& u, int c0, int lane, float (*rows)[D + 4]) {
     constexpr int E = D / 16;
     const int G = a.hq / a.hkv, l16 = lane & 15, g = lane >> 4, n = lane & 15;
-    qlarge = false;
+    qlarge = 0;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       float inv = 1.f;
@@ -295,17 +302,18 @@ struct TreeWave {
       }
       __asm__ volatile("" ::: "memory");
       qs[ct] = inv;
-      qlarge = qlarge || __builtin_amdgcn_ballot_w64(inv != 1.f) != 0;
+      qlarge |= __builtin_amdgcn_ballot_w64(inv != 1.f) != 0 ? 1 : 0;
     }
   }
 
   // One tile of the positions from pos0 on: kb, vb, xb its operands ([k][part][NS],
   // [p][part][NB] and [p] units of 64), tb its factors.  edge (uniform): some column
   // does not attend all of it, or (bit k of `on`: positions 16 k .. have a page) nobody
-  // some.  next(): called behind the score products.
+  // some.  beside(0), beside(1): work to do under the score products and under the
+  // value products.
   template <typename F>
   __device__ __forceinline__ void tile(const TreeArgs& a, const TreeUnit& u, const u32x4* kb, const u32x4* vb, const u32x4* xb,
-                                       const float (*tb)[TK], int pos0, bool edge, uint32_t on, int lane, F next) {
+                                       const float (*tb)[TK], int pos0, bool edge, uint32_t on, int lane, F beside) {
     const int g = lane >> 4;
     floatx4 s[NT][CT];
 #pragma unroll
@@ -346,7 +354,7 @@ struct TreeWave {
           for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[d][k], qh[ct][d0 + d], s[k][ct], 0, 0, 0);
       }
     }
-    next();
+    beside(std::integral_constant<int, 0>{});
     float tf[2][NT][4];  // the factors of this lane's positions 16 k + 4 g + i
 #pragma unroll
     for (int f = 0; f < 2; ++f)
@@ -355,7 +363,7 @@ struct TreeWave {
         const float4 x = *reinterpret_cast<const float4*>(&tb[f][16 * k + 4 * g]);
         tf[f][k][0] = x.x; tf[f][k][1] = x.y; tf[f][k][2] = x.z; tf[f][k][3] = x.w;
       }
-    if (qlarge) {
+    if (qlarge != 0) {
 #pragma unroll
       for (int k = 0; k < NT; ++k)
 #pragma unroll
@@ -383,13 +391,11 @@ struct TreeWave {
               if (((vis >> (16 * k + i)) & 1u) == 0) y[2 * p + k][ct][i] = -INFINITY;
         }
     }
-    float tm = y[0][0][0];
+    float tm = -INFINITY;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-      for (int k = 0; k < NT; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tm = fmaxf(tm, y[k][ct][i]);
+      for (int k = 0; k < NT; ++k) tm = tree_max3(tree_max3(tm, y[k][ct][0], y[k][ct][1]), y[k][ct][2], y[k][ct][3]);
     if (__builtin_amdgcn_ballot_w64(tm > TAU) != 0) {  // wave-uniform, rare: raise the maxima
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
@@ -441,21 +447,26 @@ struct TreeWave {
       if constexpr (NH == 2) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, of(pl[p][ct], swap), c, 0, 0, 0);
       c = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, of(ph[p][ct], swap), c, 0, 0, 0);
     };
+    half8 xx[NP], xv[NP * NB];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) xx[p] = __builtin_bit_cast(half8, xb[p * 64 + lane]);
+#pragma unroll
+    for (int i = 0; i < NP * NB; ++i) xv[i] = __builtin_bit_cast(half8, vb[((i / NB) * VP * NB + i % NB) * 64 + lane]);
+    __builtin_amdgcn_sched_barrier(0);
+    beside(std::integral_constant<int, 1>{});
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      const half8 x = __builtin_bit_cast(half8, xb[p * 64 + lane]);
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) product(x, accx[ct], p, ct, false);
+      for (int ct = 0; ct < CT; ++ct) product(xx[p], accx[ct], p, ct, false);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const half8 v = __builtin_bit_cast(half8, vb[(p * VP * NB + b) * 64 + lane]);
         if constexpr (VHL) {
           const half8 lo = __builtin_bit_cast(half8, vb[((p * VP + 1) * NB + b) * 64 + lane]);
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, of(ph[p][ct], C::vx(b)), acc[ct][b], 0, 0, 0);
         }
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) product(v, acc[ct][b], p, ct, C::vx(b));
+        for (int ct = 0; ct < CT; ++ct) product(xv[p * NB + b], acc[ct][b], p, ct, C::vx(b));
       }
     }
   }
@@ -466,8 +477,8 @@ struct TreeWave {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       // sums of the weights and of the minima, both times LIFT, from the lanes g = 0
-      const float L = __shfl(__builtin_fmaf(accx[ct][1], 1.f / 2048.f, accx[ct][0]), n) * (1.f / 32.f);
-      const float Z = __shfl(__builtin_fmaf(accx[ct][3], 1.f / 2048.f, accx[ct][2]), n) * 16.f;
+      const float L = __shfl(__builtin_fmaf(accx[ct][2], 1.f / 2048.f, accx[ct][0]), n) * (1.f / 32.f);
+      const float Z = __shfl(__builtin_fmaf(accx[ct][3], 1.f / 2048.f, accx[ct][1]), n) * 16.f;
       const bool none = L == 0.f;  // no position; a NaN score makes L, and the output, NaN
       const float inv = none ? 0.f : 1.f / L;
       float y[4][NB];

@@ -11,9 +11,9 @@ namespace ftq {
 
 float fwht_scale(int d);
 bool v1_widths_ok(int kb, int vb, int flags);
-hipError_t tree_fast_64(const TreeArgs& a, unsigned grid, hipStream_t st);
-hipError_t tree_fast_128(const TreeArgs& a, unsigned grid, hipStream_t st);
-hipError_t tree_fast_256(const TreeArgs& a, unsigned grid, hipStream_t st);
+hipError_t tree_fast_64(const TreeArgs& a, int ct, unsigned grid, hipStream_t st);
+hipError_t tree_fast_128(const TreeArgs& a, int ct, unsigned grid, hipStream_t st);
+hipError_t tree_fast_256(const TreeArgs& a, int ct, unsigned grid, hipStream_t st);
 
 namespace {
 
@@ -92,11 +92,10 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
   }
 
   for (int blk = u.blk; blk * 64 * CT < u.n * G; blk += a.nblk) {
-    const int c0 = blk * 64 * CT + wave * 16 * CT;
     W w;
     int first, last;
-    w.columns(a, u, c0, lane, wave, red, u.len, first, last);  // its barrier: the pool is free, and the tables written
-    w.queries(a, u, c0, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
+    w.columns(a, u, blk, lane, wave, red, u.len, first, last);  // its barrier: the pool is free, and the tables written
+    w.queries(a, u, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
     __syncthreads();
     first = min(first, u.ctx);  // the tree's own positions always
     const int held = (int)min((int64_t)u.len, (int64_t)a.max_blocks << a.lbs);  // positions that can have a page
@@ -216,10 +215,10 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
       }
       __syncthreads();
       const uint32_t on = tree_held<TK>(a, u, pos0);  // bit k: positions 16 k .. of the tile have a page
-      w.tile(a, u, kf, vf, xb, tb, pos0, pos0 < last || pos0 + TK > u.ctx || on != (1u << NT) - 1u, on, lane, [](auto) {});
+      w.step(a, u, kf, vf, xb, tb, pos0, pos0 < last || pos0 + TK > u.ctx || on != (1u << NT) - 1u, on, lane, [](auto) {});
       __syncthreads();  // before the next tile's rows
     }
-    w.finish(a, u, c0, lane);
+    w.finish(a, u, lane);
   }
 }
 
@@ -260,16 +259,18 @@ bool tree_fast_takes(const TreeArgs& a) {
 }
 
 template <int D>
-hipError_t tree_launch(const TreeArgs& a, int64_t tokens, bool vrot, hipStream_t st) {
+hipError_t tree_launch(const TreeArgs& a, int ct, int64_t tokens, bool vrot, hipStream_t st) {
   const unsigned grid = (unsigned)((int64_t)a.nblk * a.splits * a.B * a.hkv);
   const bool lm = (a.flags & V1F_VLM) != 0 && a.vb == 4;
-  const hipError_t e = tree_fast_takes(a) ? (D == 64 ? tree_fast_64(a, grid, st) : D == 128 ? tree_fast_128(a, grid, st) : tree_fast_256(a, grid, st))
+  const hipError_t e = tree_fast_takes(a) ? (D == 64 ? tree_fast_64(a, ct, grid, st) : D == 128 ? tree_fast_128(a, ct, grid, st) : tree_fast_256(a, ct, grid, st))
                        : lm ? any_launch<D, true>(a, grid, st) : any_launch<D, false>(a, grid, st);
   if (e != hipSuccess || a.wo == nullptr) return e;
   return tree_merge<D>(a, tokens, vrot, st);
 }
 
-int tree_cols(int d) { return d == 256 ? 64 : 128; }
+// 16-column tiles of a wave for sequences of at most `cols` columns: one where 64
+// columns do (fewer registers, three workgroups a CU instead of two).
+int tree_ct(int d, int64_t cols) { return d == 256 || cols <= 64 ? 1 : 2; }
 
 }  // namespace
 }  // namespace ftq
@@ -282,8 +283,9 @@ extern "C" int ftq_v1_tree_choose_splits(int batch, int max_query_len, int num_q
   if (batch <= 0 || max_query_len <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 ||
       max_seq_len <= 0)
     return 1;
-  const int cols = tree_cols(d);
-  const int64_t nblk = ((int64_t)max_query_len * (num_q_heads / num_kv_heads) + cols - 1) / cols;
+  const int64_t ncols = (int64_t)max_query_len * (num_q_heads / num_kv_heads);
+  const int cols = 64 * tree_ct(d, ncols);
+  const int64_t nblk = (ncols + cols - 1) / cols;
   const int64_t wgs = (int64_t)batch * num_kv_heads * nblk;
   const int64_t tiles = ((int64_t)max_seq_len + 31) / 32;
   const int64_t s = std::min<int64_t>(512 / std::max<int64_t>(wgs, 1), tiles / 4);
@@ -333,32 +335,33 @@ extern "C" int ftq_v1_tree_attention(const void* query, int q_dtype, int64_t num
   FTQ_REQUIRE(((uintptr_t)tree_mask & 7u) == 0, "tree_mask must be 8-byte aligned");
   const int64_t need = split_workspace_bytes((int)num_tokens, num_q_heads, d, num_splits);
   FTQ_REQUIRE(need >= 0 && workspace_bytes >= need, "workspace too small (see ftq_v1_workspace_bytes)");
-  const int G = num_q_heads / num_kv_heads, cols = tree_cols(d);
-  const int64_t mq = std::min<int64_t>(max_query_len, num_tokens);
-  const int64_t nblk = (mq * G + cols - 1) / cols;
+  const int64_t ncols = std::min<int64_t>(max_query_len, num_tokens) * (num_q_heads / num_kv_heads);
+  TreeArgs a{};
+  a.ot = out_dtype; a.kb = key_bits; a.vb = value_bits; a.flags = v_flags;
+  a.cache = kv_cache; a.nb = num_blocks; a.sblk = stride_block; a.spos = stride_pos; a.shead = stride_head;
+  const int ct = tree_fast_takes(a) ? tree_ct(d, ncols) : tree_ct(d, INT32_MAX);
+  const int64_t nblk = (ncols + 64 * ct - 1) / (64 * ct);
   int64_t grid = 0;
   FTQ_REQUIRE(!__builtin_mul_overflow(nblk * num_splits, (int64_t)batch * num_kv_heads, &grid) && grid <= INT32_MAX,
               "tree attention: grid too large");
   const bool vrot = (v_flags & V1F_VROT) != 0;
-  TreeArgs a{};
   a.q = query; a.qt = q_dtype; a.tokens = (int)num_tokens;
-  a.cache = kv_cache; a.nb = num_blocks; a.sblk = stride_block; a.spos = stride_pos; a.shead = stride_head;
   while ((1 << a.lbs) < block_size) ++a.lbs;
   a.bt = block_table; a.max_blocks = max_blocks_per_seq;
   a.sl = seq_lens; a.qsl = query_start_loc; a.ks = kv_start;
   a.mask = tree_mask; a.words = mask_words;
   a.B = batch; a.hq = num_q_heads; a.hkv = num_kv_heads;
-  a.cent = centroids; a.kb = key_bits; a.vb = value_bits; a.flags = v_flags;
+  a.cent = centroids;
   a.qscale = (raw || rotation != nullptr ? 1.f : fwht_scale(d)) * scale * 1.4426950408889634f;
   a.splits = num_splits; a.nblk = (int)nblk;
   const bool direct = num_splits == 1 && !(vrot && rotation != nullptr);
   a.wo = direct ? nullptr : static_cast<float*>(workspace);
   a.wl = direct ? nullptr : a.wo + num_tokens * num_q_heads * num_splits * d;
-  a.out = out; a.ot = out_dtype;
+  a.out = out;
   a.unrot = vrot; a.oscale = vrot ? fwht_scale(d) : 1.f;
   a.lse = lse_out; a.rot = rotation;
   hipStream_t st = (hipStream_t)stream;
-  const hipError_t e = d == 64 ? tree_launch<64>(a, num_tokens, vrot, st) : d == 128 ? tree_launch<128>(a, num_tokens, vrot, st)
-                                                                                    : tree_launch<256>(a, num_tokens, vrot, st);
+  const hipError_t e = d == 64 ? tree_launch<64>(a, ct, num_tokens, vrot, st) : d == 128 ? tree_launch<128>(a, ct, num_tokens, vrot, st)
+                                                                                    : tree_launch<256>(a, ct, num_tokens, vrot, st);
   return hip_status(e);
 }

@@ -2,5 +2,5 @@
 #include "ftq_tree_fast.h"
 
 namespace ftq {
-hipError_t tree_fast_128(const TreeArgs& a, unsigned grid, hipStream_t st) { return tree_fast_launch<128>(a, grid, st); }
+hipError_t tree_fast_128(const TreeArgs& a, int ct, unsigned grid, hipStream_t st) { return tree_fast_launch<128>(a, ct, grid, st); }
 }  // namespace ftq

@@ -2,5 +2,5 @@
 #include "ftq_tree_fast.h"
 
 namespace ftq {
-hipError_t tree_fast_64(const TreeArgs& a, unsigned grid, hipStream_t st) { return tree_fast_launch<64>(a, grid, st); }
+hipError_t tree_fast_64(const TreeArgs& a, int ct, unsigned grid, hipStream_t st) { return tree_fast_launch<64>(a, ct, grid, st); }
 }  // namespace ftq

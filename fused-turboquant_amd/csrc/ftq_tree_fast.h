@@ -231,11 +231,11 @@ struct TreeFmt {
   }
 };
 
-template <int D, int KB, int VB, int NH>
-__global__ __launch_bounds__(256, 2) void tree_fast_kernel(const TreeArgs a) {
+template <int D, int KB, int VB, int NH, int CT>
+__global__ __launch_bounds__(256, D == 128 && CT == 1 ? 3 : 2) void tree_fast_kernel(const TreeArgs a) {
   using C = TreeGeo<D>;
   using F = TreeFmt<D, KB, VB>;
-  constexpr int CT = C::CT, TK = C::TK, NT = C::NT, NP = C::NP;
+  constexpr int TK = C::TK, NT = C::NT, NP = C::NP;
   using W = TreeWave<D, CT, false, NH, false>;
   using B = TreeBuf<D>;
   constexpr int QU = 64 * (D + 4) / 4;
@@ -260,14 +260,9 @@ __global__ __launch_bounds__(256, 2) void tree_fast_kernel(const TreeArgs a) {
   const uint8_t* head = a.cache + (int64_t)u.kvh * a.shead + (int64_t)within * a.spos;
 
   for (int blk = u.blk; blk * 64 * CT < u.n * G; blk += a.nblk) {
-    const int c0 = blk * 64 * CT + wave * 16 * CT;
     W w;
     int first, last;
-    w.columns(a, u, c0, lane, wave, red, u.len, first, last);  // its barrier: the pool is free
-    w.queries(a, u, c0, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
-    __syncthreads();
-    if (tid < 2 * 64 * NP) pool[tid / (64 * NP) * B::SIZE + B::X + tid % (64 * NP)] = u32x4{0, 0, 0, 0};
-    __syncthreads();
+    w.columns(a, u, blk, lane, wave, red, u.len, first, last);  // its barrier: the pool is free
     first = min(first, u.ctx);  // the tree's own positions always
     const int held = (int)min((int64_t)u.len, (int64_t)a.max_blocks << a.lbs);  // positions that can have a page
     const int t0 = first / TK, t1 = max((held + TK - 1) / TK, t0);
@@ -293,48 +288,77 @@ __global__ __launch_bounds__(256, 2) void tree_fast_kernel(const TreeArgs a) {
       entries(min(t + 1, tb1 - 1));
     };
     uint32_t now = 0;  // `on` of the tile that is multiplied
-    if (tb0 < tb1) {
+    if (tb0 < tb1) {  // the first bytes are on their way while the queries are rotated
       entries(tb0);
       fetch(tb0);
+    }
+    w.queries(a, u, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
+    __syncthreads();
+    if (tid < 2 * 64 * NP) pool[tid / (64 * NP) * B::SIZE + B::X + tid % (64 * NP)] = u32x4{0, 0, 0, 0};
+    __syncthreads();
+    if (tb0 < tb1) {
       raw.emit_k(table, pool, wave, lane);
       raw.emit_v(pool, wave, lane);
       now = on;
       fetch(min(tb0 + 1, tb1 - 1));
     }
-    int p = 0;
-    for (int t = tb0; t < tb1; ++t, p ^= 1) {
-      tree_barrier();
-      const int pos0 = t * TK;
-      const u32x4* buf = pool + p * B::SIZE;
-      u32x4* to = pool + (p ^ 1) * B::SIZE;
-      // (behind the last tile: it again, for nobody)
-      auto beside = [&](auto part) __attribute__((always_inline)) {
-        if constexpr (decltype(part)::value == 0) raw.emit_k(table, to, wave, lane);
-        else raw.emit_v(to, wave, lane);
-      };
-      w.tile(a, u, buf, buf + B::V, buf + B::X, reinterpret_cast<const float(*)[TK]>(buf + B::T), pos0,
-             pos0 < last || pos0 + TK > u.ctx || now != (1u << NT) - 1u, now, lane, beside);
-      now = on;
-      fetch(min(t + 2, tb1 - 1));
-    }
-    w.finish(a, u, c0, lane);
+    // A loop for each number of column tiles in use: every wave meets the others'
+    // barriers in its own (a branch inside one loop costs copies of the accumulators).
+    auto run = [&](auto use) __attribute__((always_inline)) {
+      constexpr int USE = decltype(use)::value;
+      int p = 0;
+      for (int t = tb0; t < tb1; ++t, p ^= 1) {
+        tree_barrier();
+        const int pos0 = t * TK;
+        const u32x4* buf = pool + p * B::SIZE;
+        u32x4* to = pool + (p ^ 1) * B::SIZE;
+        // (behind the last tile: it again, for nobody)
+        auto beside = [&](auto part) __attribute__((always_inline)) {
+          if constexpr (decltype(part)::value == 0) raw.emit_k(table, to, wave, lane);
+          else raw.emit_v(to, wave, lane);
+        };
+        if constexpr (USE > 0) {
+          w.template tile<USE>(a, u, buf, buf + B::V, buf + B::X, reinterpret_cast<const float(*)[TK]>(buf + B::T), pos0,
+                               pos0 < last || pos0 + TK > u.ctx || now != (1u << NT) - 1u, now, lane, beside);
+        } else {
+          beside(std::integral_constant<int, 0>{});
+          beside(std::integral_constant<int, 1>{});
+        }
+        now = on;
+        fetch(min(t + 2, tb1 - 1));
+      }
+    };
+    if (CT > 1 && w.nct > 1) run(std::integral_constant<int, CT>{});
+    else if (w.nct == 1) run(std::integral_constant<int, 1>{});
+    else run(std::integral_constant<int, 0>{});
+    w.finish(a, u, lane);
   }
 }
 
-template <int D, int KB, int VB>
-hipError_t tree_fast_go(const TreeArgs& a, unsigned grid, hipStream_t st) {
-  if (a.ot == BF16) tree_fast_kernel<D, KB, VB, 1><<<dim3(grid), dim3(256), 0, st>>>(a);
-  else tree_fast_kernel<D, KB, VB, 2><<<dim3(grid), dim3(256), 0, st>>>(a);
+template <int D, int KB, int VB, int NH>
+hipError_t tree_fast_ct(const TreeArgs& a, int ct, unsigned grid, hipStream_t st) {
+  if constexpr (D != 256) {
+    if (ct == 2) {
+      tree_fast_kernel<D, KB, VB, NH, 2><<<dim3(grid), dim3(256), 0, st>>>(a);
+      return hipGetLastError();
+    }
+  }
+  tree_fast_kernel<D, KB, VB, NH, 1><<<dim3(grid), dim3(256), 0, st>>>(a);
   return hipGetLastError();
 }
+template <int D, int KB, int VB>
+hipError_t tree_fast_go(const TreeArgs& a, int ct, unsigned grid, hipStream_t st) {
+  return a.ot == BF16 ? tree_fast_ct<D, KB, VB, 1>(a, ct, grid, st) : tree_fast_ct<D, KB, VB, 2>(a, ct, grid, st);
+}
 
+// ct: 16-column tiles of a wave
 template <int D>
-hipError_t tree_fast_launch(const TreeArgs& a, unsigned grid, hipStream_t st) {
-  if (a.kb == TREE_RAW) return tree_fast_go<D, TREE_RAW, TREE_RAW>(a, grid, st);
-#define FTQ_TREE_VB(KB)                                     \
-  return a.vb == 2   ? tree_fast_go<D, KB, 2>(a, grid, st) \
-         : a.vb == 3 ? tree_fast_go<D, KB, 3>(a, grid, st) \
-                     : tree_fast_go<D, KB, 4>(a, grid, st)
+hipError_t tree_fast_launch(const TreeArgs& a, int ct, unsigned grid, hipStream_t st) {
+  if (a.kb == TREE_RAW) return tree_fast_go<D, TREE_RAW, TREE_RAW>(a, ct, grid, st);
+#define FTQ_TREE_VB(KB)                                         \
+  return a.vb == 2   ? tree_fast_go<D, KB, 2>(a, ct, grid, st) \
+         : a.vb == 3 ? tree_fast_go<D, KB, 3>(a, ct, grid, st) \
+                     : tree_fast_go<D, KB, 4>(a, ct, grid, st)
   if (a.kb == 2) FTQ_TREE_VB(2);
   if (a.kb == 3) FTQ_TREE_VB(3);
   FTQ_TREE_VB(4);

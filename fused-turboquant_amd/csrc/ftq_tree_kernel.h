@@ -68,7 +68,7 @@ struct TreeArgs {
 constexpr int TREE_RAW = 16;  // key_bits of raw fp16 slots
 
 template <int D> struct TreeGeo {
-  static constexpr int CT = D == 256 ? 1 : 2;     // 16-column tiles per wave
+  static constexpr int CT = D == 256 ? 1 : 2;     // 16-column tiles per wave, at most
   static constexpr int TK = D == 64 ? 64 : 32;    // positions of a tile
   static constexpr int NS = D / 32, NB = D / 16, NT = TK / 16, NP = TK / 32;
   // The dequantising lanes of one position write the steps and rows (s, g) of one m,
@@ -199,24 +199,32 @@ struct TreeWave {
   static constexpr float TAU = 4.f;        // weights stay below 2^TAU
   static constexpr float MINF = -3.0e38f;  // running maximum of a column with no position yet
 
+  // (the scalars apart from each other: neighbours would be loaded together before
+  // they are registers, and then never become any)
+  int c0, nct;                             // the wave's first column; tiles of columns in use (uniform; 0: none)
+  int qlarge;                              // some qs is not 1 (wave-uniform)
   half8 qh[CT][NS], ql[NH == 2 ? CT : 1][NH == 2 ? NS : 1];
   float qs[CT];                            // of the scores: 1, or what a query beyond f16's range was divided by
-  int qlarge;                              // some qs is not 1 (wave-uniform)
+  floatx4 acc[CT][NB];
   float m_run[CT];
-  floatx4 acc[CT][NB], accx[CT];           // accx: lanes of row 0: the rows of X
+  floatx4 accx[CT];                        // lanes of row 0: the rows of X
   int row[CT];                             // query row in the sequence, or -1
 
   // The columns, and the first and last of their first context positions over the
   // workgroup (`none` and 0 for a wave without columns)
-  __device__ __forceinline__ void columns(const TreeArgs& a, const TreeUnit& u, int c0, int lane, int wave, int (*red)[2],
+  __device__ __forceinline__ void columns(const TreeArgs& a, const TreeUnit& u, int blk, int lane, int wave, int (*red)[2],
                                           int none, int& first, int& last) {
-    const int G = a.hq / a.hkv, n = lane & 15;
+    const int G = a.hq / a.hkv, n = lane & 15, begin = blk * 64 * CT;
+    // a block of at most 64 columns is one tile of each wave
+    const int each = CT > 1 && u.n * G - begin <= 64 ? 1 : CT;
+    c0 = begin + wave * 16 * each;
+    nct = __builtin_amdgcn_readfirstlane(min(max((u.n * G - c0 + 15) / 16, 0), each));
     first = none;
     last = 0;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       const int col = c0 + 16 * ct + n;
-      row[ct] = col < u.n * G ? col / G : -1;
+      row[ct] = ct < each && col < u.n * G ? col / G : -1;
       if (row[ct] >= 0) {
         const int start = a.ks != nullptr ? max(a.ks[u.q0 + row[ct]], 0) : 0;
         first = min(first, start);
@@ -240,54 +248,57 @@ struct TreeWave {
 
   // The columns' queries, rotated and scaled, as f16 hi + lo.  One query per 16
   // lanes, four at a time, through 16 rows of LDS of the wave's own.
-  __device__ __forceinline__ void queries(const TreeArgs& a, const TreeUnit& u, int c0, int lane, float (*rows)[D + 4]) {
+  __device__ __forceinline__ void queries(const TreeArgs& a, const TreeUnit& u, int lane, float (*rows)[D + 4]) {
     constexpr int E = D / 16;
     const int G = a.hq / a.hkv, l16 = lane & 15, g = lane >> 4, n = lane & 15;
     qlarge = 0;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       float inv = 1.f;
-#pragma unroll 1
-      for (int k = 0; k < 4; ++k) {
-        const int col = c0 + 16 * ct + 4 * k + g;
-        const bool on = col < u.n * G;
-        const int r = on ? col / G : 0, h = u.kvh * G + (on ? col - r * G : 0);
-        float y[E];
+      if (ct < nct) {
+        float y[4][E];  // all four loads at once
 #pragma unroll
-        for (int i = 0; i < E; ++i) y[i] = 0.f;
-        if (on) {
+        for (int k = 0; k < 4; ++k) {
+          const int col = c0 + 16 * ct + 4 * k + g;
+          const bool on = col < u.n * G;
+          const int r = on ? col / G : 0, h = u.kvh * G + (on ? col - r * G : 0);
           const int64_t off = ((int64_t)(u.q0 + r) * a.hq + h) * D + l16 * E;
-          if (a.qt == F32) load_elems<F32, E>(a.q, off, y);
-          else if (a.qt == F16) load_elems<F16, E>(a.q, off, y);
-          else load_elems<BF16, E>(a.q, off, y);
-        }
-        if (a.kb != TREE_RAW) {
-          if (a.rot != nullptr) rot_matrix_lanes<D, E>(y, a.rot, rows[4 * k + g], l16);
-          else fwht_lanes<E, 16>(y, l16);
-        }
-        float mx = 0.f;
+          if (a.qt == F32) load_elems<F32, E>(a.q, off, y[k]);
+          else if (a.qt == F16) load_elems<F16, E>(a.q, off, y[k]);
+          else load_elems<BF16, E>(a.q, off, y[k]);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          y[i] *= a.qscale;
-          mx = fmaxf(mx, fabsf(y[i]));
+          for (int i = 0; i < E; ++i) y[k][i] = on ? y[k][i] : 0.f;
         }
-        mx = fmaxf(mx, lane_xor<1>(mx));
-        mx = fmaxf(mx, lane_xor<2>(mx));
-        mx = fmaxf(mx, lane_xor<4>(mx));
-        mx = fmaxf(mx, lane_xor<8>(mx));
-        // A query that f16 cannot hold is scaled to [2^13, 2^14).  Small ones need
-        // no scale: what their low parts lose below f16's range is 2^-25 of a
-        // score, an absolute error.
-        const int e = (int)((__float_as_uint(mx) >> 23) & 255u);
-        const int ue = e >= 127 + 14 && e < 255 ? 140 + 127 - e : 127;
-        const float up = __uint_as_float((uint32_t)ue << 23);
-        const float down = __uint_as_float((uint32_t)(254 - ue) << 23);
-        const float got = __shfl(down, (n & 3) << 4);  // of column 4 k + (n & 3)
-        if ((n >> 2) == k) inv = got;
 #pragma unroll
-        for (int i = 0; i < E; ++i) rows[4 * k + g][l16 * E + i] = y[i] * up;
+        for (int k = 0; k < 4; ++k) {
+          if (a.kb != TREE_RAW) {
+            if (a.rot != nullptr) rot_matrix_lanes<D, E>(y[k], a.rot, rows[4 * k + g], l16);
+            else fwht_lanes<E, 16>(y[k], l16);
+          }
+          float mx = 0.f;
+#pragma unroll
+          for (int i = 0; i < E; ++i) {
+            y[k][i] *= a.qscale;
+            mx = fmaxf(mx, fabsf(y[k][i]));
+          }
+          mx = fmaxf(mx, lane_xor<1>(mx));
+          mx = fmaxf(mx, lane_xor<2>(mx));
+          mx = fmaxf(mx, lane_xor<4>(mx));
+          mx = fmaxf(mx, lane_xor<8>(mx));
+          // A query that f16 cannot hold is scaled to [2^13, 2^14).  Small ones need
+          // no scale: what their low parts lose below f16's range is 2^-25 of a
+          // score, an absolute error.
+          const int e = (int)((__float_as_uint(mx) >> 23) & 255u);
+          const int ue = e >= 127 + 14 && e < 255 ? 140 + 127 - e : 127;
+          const float up = __uint_as_float((uint32_t)ue << 23);
+          const float down = __uint_as_float((uint32_t)(254 - ue) << 23);
+          const float got = __shfl(down, (n & 3) << 4);  // of column 4 k + (n & 3)
+          if ((n >> 2) == k) inv = got;
+#pragma unroll
+          for (int i = 0; i < E; ++i) rows[4 * k + g][l16 * E + i] = y[k][i] * up;
+        }
+        __asm__ volatile("" ::: "memory");  // a wave's LDS accesses run in order
       }
-      __asm__ volatile("" ::: "memory");  // a wave's LDS accesses run in order
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         uint32_t h[4], l[4];
@@ -310,16 +321,16 @@ struct TreeWave {
   // [p][part][NB] and [p] units of 64), tb its factors.  edge (uniform): some column
   // does not attend all of it, or (bit k of `on`: positions 16 k .. have a page) nobody
   // some.  beside(0), beside(1): work to do under the score products and under the
-  // value products.
-  template <typename F>
+  // value products.  USE: 16-column tiles in use.
+  template <int USE, typename F>
   __device__ __forceinline__ void tile(const TreeArgs& a, const TreeUnit& u, const u32x4* kb, const u32x4* vb, const u32x4* xb,
                                        const float (*tb)[TK], int pos0, bool edge, uint32_t on, int lane, F beside) {
     const int g = lane >> 4;
-    floatx4 s[NT][CT];
+    floatx4 s[NT][USE];
 #pragma unroll
     for (int k = 0; k < NT; ++k)
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) s[k][ct] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int ct = 0; ct < USE; ++ct) s[k][ct] = floatx4{0.f, 0.f, 0.f, 0.f};
     constexpr int AHEAD = KHL ? 1 : NS;  // steps whose K operands are requested together
 #pragma unroll
     for (int d0 = 0; d0 < NS; d0 += AHEAD) {
@@ -340,18 +351,18 @@ struct TreeWave {
 #pragma unroll
           for (int k = 0; k < NT; ++k)
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[d][k], ql[ct][d0 + d], s[k][ct], 0, 0, 0);
+            for (int ct = 0; ct < USE; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[d][k], ql[ct][d0 + d], s[k][ct], 0, 0, 0);
         }
         if constexpr (KHL) {
 #pragma unroll
           for (int k = 0; k < NT; ++k)
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl[d][k], qh[ct][d0 + d], s[k][ct], 0, 0, 0);
+            for (int ct = 0; ct < USE; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl[d][k], qh[ct][d0 + d], s[k][ct], 0, 0, 0);
         }
 #pragma unroll
         for (int k = 0; k < NT; ++k)
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[d][k], qh[ct][d0 + d], s[k][ct], 0, 0, 0);
+          for (int ct = 0; ct < USE; ++ct) s[k][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[d][k], qh[ct][d0 + d], s[k][ct], 0, 0, 0);
       }
     }
     beside(std::integral_constant<int, 0>{});
@@ -367,18 +378,18 @@ struct TreeWave {
 #pragma unroll
       for (int k = 0; k < NT; ++k)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) s[k][ct] *= qs[ct];
+        for (int ct = 0; ct < USE; ++ct) s[k][ct] *= qs[ct];
     }
-    floatx4 y[NT][CT];  // scores less the running maximum
+    floatx4 y[NT][USE];  // scores less the running maximum
 #pragma unroll
     for (int k = 0; k < NT; ++k)
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
+      for (int ct = 0; ct < USE; ++ct)
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[k][ct][i] = __builtin_fmaf(s[k][ct][i], tf[0][k][i], -m_run[ct]);
     if (edge) {
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
+      for (int ct = 0; ct < USE; ++ct)
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
           const uint32_t held = ((on >> (2 * p)) & 1u ? 0xffffu : 0u) | ((on >> (2 * p + 1)) & 1u ? 0xffff0000u : 0u);
@@ -393,12 +404,12 @@ struct TreeWave {
     }
     float tm = -INFINITY;
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
+    for (int ct = 0; ct < USE; ++ct)
 #pragma unroll
       for (int k = 0; k < NT; ++k) tm = tree_max3(tree_max3(tm, y[k][ct][0], y[k][ct][1]), y[k][ct][2], y[k][ct][3]);
     if (__builtin_amdgcn_ballot_w64(tm > TAU) != 0) {  // wave-uniform, rare: raise the maxima
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
+      for (int ct = 0; ct < USE; ++ct) {
         float mx = -INFINITY;
 #pragma unroll
         for (int k = 0; k < NT; ++k)
@@ -420,10 +431,10 @@ struct TreeWave {
       }
     }
     // weights x V factor as f16 parts
-    u32x4 ph[NP][CT], pl[NH == 2 ? NP : 1][NH == 2 ? CT : 1];
+    u32x4 ph[NP][USE], pl[NH == 2 ? NP : 1][NH == 2 ? USE : 1];
     auto weights = [&](auto masked) __attribute__((always_inline)) {
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
+      for (int ct = 0; ct < USE; ++ct)
 #pragma unroll
         for (int k = 0; k < NT; ++k) {
           float w[4];
@@ -457,22 +468,36 @@ struct TreeWave {
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) product(xx[p], accx[ct], p, ct, false);
+      for (int ct = 0; ct < USE; ++ct) product(xx[p], accx[ct], p, ct, false);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         if constexpr (VHL) {
           const half8 lo = __builtin_bit_cast(half8, vb[((p * VP + 1) * NB + b) * 64 + lane]);
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, of(ph[p][ct], C::vx(b)), acc[ct][b], 0, 0, 0);
+          for (int ct = 0; ct < USE; ++ct) acc[ct][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, of(ph[p][ct], C::vx(b)), acc[ct][b], 0, 0, 0);
         }
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) product(xv[p * NB + b], acc[ct][b], p, ct, C::vx(b));
+        for (int ct = 0; ct < USE; ++ct) product(xv[p * NB + b], acc[ct][b], p, ct, C::vx(b));
       }
     }
   }
 
+  // tile<> for the tiles in use; a wave without columns does its share of the work beside
+  template <typename F>
+  __device__ __forceinline__ void step(const TreeArgs& a, const TreeUnit& u, const u32x4* kb, const u32x4* vb, const u32x4* xb,
+                                       const float (*tb)[TK], int pos0, bool edge, uint32_t on, int lane, F beside) {
+    if (CT > 1 && nct > 1) {
+      tile<CT>(a, u, kb, vb, xb, tb, pos0, edge, on, lane, beside);
+    } else if (nct == 1) {
+      tile<1>(a, u, kb, vb, xb, tb, pos0, edge, on, lane, beside);
+    } else {
+      beside(std::integral_constant<int, 0>{});
+      beside(std::integral_constant<int, 1>{});
+    }
+  }
+
   // Lane (n, g) holds dims NB (4 g + i) + b of column n.
-  __device__ __forceinline__ void finish(const TreeArgs& a, const TreeUnit& u, int c0, int lane) {
+  __device__ __forceinline__ void finish(const TreeArgs& a, const TreeUnit& u, int lane) {
     const int n = lane & 15, g = lane >> 4, G = a.hq / a.hkv;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {

@@ -103,8 +103,7 @@ __global__ __launch_bounds__(256) void merge_splits_kernel(const float* __restri
                                                            int64_t rows, int num_splits,
                                                            const float* __restrict__ signs,
                                                            float scale, void* __restrict__ out,
-                                                           float* __restrict__ lse_out,
-                                                           const int32_t* __restrict__ end, int per) {
+                                                           float* __restrict__ lse_out) {
   static_assert(WPR == 1 || WPR == 4, "one or four waves per row");
   constexpr int E = D / 64;
   constexpr int RPB = 4 / WPR;  // rows per workgroup
@@ -112,7 +111,6 @@ __global__ __launch_bounds__(256) void merge_splits_kernel(const float* __restri
   __shared__ float wpart[4];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int64_t r = (int64_t)blockIdx.x * RPB + (WPR == 4 ? 0 : wv);
-  if (end != nullptr) rows = min(rows, (int64_t)*end * per);
   const bool live = r < rows;  // uniform per wave (and per workgroup when WPR == 4)
   const float* lse = ws_lse + (live ? r : 0) * num_splits;
 
@@ -212,18 +210,17 @@ __global__ __launch_bounds__(256) void merge_splits_kernel(const float* __restri
 }
 
 // Launch helper: four waves per row when there are enough splits to share.
-// end: device count of the `per`-row groups that are written (null: all rows).
 template <int D, int OT, int ROT>
 hipError_t launch_merge_splits(const float* ws_o, const float* ws_lse, int64_t rows, int num_splits,
                                const float* signs, float scale, void* out, hipStream_t st,
-                               float* lse_out = nullptr, const int32_t* end = nullptr, int per = 1) {
+                               float* lse_out = nullptr) {
   if (rows <= 0) return hipSuccess;
   if (num_splits >= 8) {
     merge_splits_kernel<D, OT, ROT, 4><<<dim3((unsigned)rows), dim3(256), 0, st>>>(
-        ws_o, ws_lse, rows, num_splits, signs, scale, out, lse_out, end, per);
+        ws_o, ws_lse, rows, num_splits, signs, scale, out, lse_out);
   } else {
     merge_splits_kernel<D, OT, ROT, 1><<<dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st>>>(
-        ws_o, ws_lse, rows, num_splits, signs, scale, out, lse_out, end, per);
+        ws_o, ws_lse, rows, num_splits, signs, scale, out, lse_out);
   }
   return hipGetLastError();
 }

@@ -59,9 +59,11 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
   __shared__ float table_scale_inv;
   __shared__ int red[4][2];
 
-  const TreeUnit u(a);
   const int G = a.hq / a.hkv, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  TreeUnit u;
+  TreePart part;
+  if (!tree_share<TK>(a, lane, u, part)) return;
   const bool raw = a.kb == TREE_RAW, kf8 = (a.flags & V1F_KFP8) != 0;
   const V1Geom geo = raw ? V1Geom{2 * D, 2 * D, 2 * D, 4 * D} : v1_geom(D, a.kb, a.vb, kf8);
   const int nd = (geo.raw + 3) / 4, pitch = (nd + 1) | 1;
@@ -91,17 +93,14 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
     if (lane == 0) table_scale_inv = 1.f / sg;
   }
 
-  for (int blk = u.blk; blk * 64 * CT < u.n * G; blk += a.nblk) {
+  for (; part.blk * 64 * CT < u.n * G; part.blk += a.nblk) {
     W w;
     int first, last;
-    w.columns(a, u, blk, lane, wave, red, u.len, first, last);  // its barrier: the pool is free, and the tables written
+    w.columns(a, u, part.blk, lane, wave, red, u.len, first, last);  // its barrier: the pool is free, and the tables written
     w.queries(a, u, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
     __syncthreads();
-    first = min(first, u.ctx);  // the tree's own positions always
-    const int held = (int)min((int64_t)u.len, (int64_t)a.max_blocks << a.lbs);  // positions that can have a page
-    const int t0 = first / TK, t1 = max((held + TK - 1) / TK, t0);
-    const int per = (t1 - t0 + a.splits - 1) / a.splits;
-    const int tb0 = t0 + u.split * per, tb1 = min(tb0 + per, t1);
+    first = min(first, u.ctx) / TK;  // the tree's own positions always
+    const int tb0 = part.part == 0 ? first : max(part.tb0, first), tb1 = part.tb1;
 
     for (int t = tb0; t < tb1; ++t) {
       const int pos0 = t * TK;
@@ -218,7 +217,7 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
       w.step(a, u, kf, vf, xb, tb, pos0, pos0 < last || pos0 + TK > u.ctx || on != (1u << NT) - 1u, on, lane, [](auto) {});
       __syncthreads();  // before the next tile's rows
     }
-    w.finish(a, u, lane);
+    w.finish(a, u, part, lane);
   }
 }
 
@@ -237,16 +236,17 @@ hipError_t any_launch(const TreeArgs& a, unsigned grid, hipStream_t st) {
 
 template <int D>
 hipError_t tree_merge(const TreeArgs& a, int64_t tokens, bool vrot, hipStream_t st) {
-  const int64_t rows = tokens * a.hq;
-  const int32_t* end = a.qsl + a.B;  // rows behind the last sequence stay as they are
+  const dim3 grid((unsigned)((tokens * a.hq + 3) / 4)), block(256);
+  const int32_t* end = a.qsl + a.B;
   const float rs = fwht_scale(D);
-#define FTQ_TREE_MERGE(R, S, F)                                                                                          \
-  return a.ot == F32   ? launch_merge_splits<D, F32, R>(a.wo, a.wl, rows, a.splits, S, F, a.out, st, a.lse, end, a.hq) \
-         : a.ot == F16 ? launch_merge_splits<D, F16, R>(a.wo, a.wl, rows, a.splits, S, F, a.out, st, a.lse, end, a.hq) \
-                       : launch_merge_splits<D, BF16, R>(a.wo, a.wl, rows, a.splits, S, F, a.out, st, a.lse, end, a.hq)
+#define FTQ_TREE_MERGE(R, S, F)                                                                                              \
+  (a.ot == F32   ? tree_merge_kernel<D, F32, R><<<grid, block, 0, st>>>(a.wo, a.wl, end, a.tokens, a.hq, a.splits, S, F, a.out, a.lse) \
+   : a.ot == F16 ? tree_merge_kernel<D, F16, R><<<grid, block, 0, st>>>(a.wo, a.wl, end, a.tokens, a.hq, a.splits, S, F, a.out, a.lse) \
+                 : tree_merge_kernel<D, BF16, R><<<grid, block, 0, st>>>(a.wo, a.wl, end, a.tokens, a.hq, a.splits, S, F, a.out, a.lse))
   if (vrot && a.rot != nullptr) FTQ_TREE_MERGE(ROT_MATRIX, a.rot, 1.f);
-  if (vrot) FTQ_TREE_MERGE(ROT_PLAIN, nullptr, rs);
-  FTQ_TREE_MERGE(ROT_NONE, nullptr, rs);
+  else if (vrot) FTQ_TREE_MERGE(ROT_PLAIN, nullptr, rs);
+  else FTQ_TREE_MERGE(ROT_NONE, nullptr, rs);
+  return hipGetLastError();
 #undef FTQ_TREE_MERGE
 }
 
@@ -259,8 +259,7 @@ bool tree_fast_takes(const TreeArgs& a) {
 }
 
 template <int D>
-hipError_t tree_launch(const TreeArgs& a, int ct, int64_t tokens, bool vrot, hipStream_t st) {
-  const unsigned grid = (unsigned)((int64_t)a.nblk * a.splits * a.B * a.hkv);
+hipError_t tree_launch(const TreeArgs& a, int ct, unsigned grid, int64_t tokens, bool vrot, hipStream_t st) {
   const bool lm = (a.flags & V1F_VLM) != 0 && a.vb == 4;
   const hipError_t e = tree_fast_takes(a) ? (D == 64 ? tree_fast_64(a, ct, grid, st) : D == 128 ? tree_fast_128(a, ct, grid, st) : tree_fast_256(a, ct, grid, st))
                        : lm ? any_launch<D, true>(a, grid, st) : any_launch<D, false>(a, grid, st);
@@ -269,8 +268,15 @@ hipError_t tree_launch(const TreeArgs& a, int ct, int64_t tokens, bool vrot, hip
 }
 
 // 16-column tiles of a wave for sequences of at most `cols` columns: one where 64
-// columns do (fewer registers, three workgroups a CU instead of two).
+// columns do (fewer registers, more workgroups a CU).
 int tree_ct(int d, int64_t cols) { return d == 256 || cols <= 64 ? 1 : 2; }
+// Parts (TreeShare) of all sequences together, per kv head and column block: what the
+// 256 CUs hold at once (three workgroups a CU at d = 128 with one column tile a wave,
+// else two); where that is hardly more than the sequences, three rounds of it or more.
+int64_t tree_parts_all(int d, int ct, int hkv, int64_t nblk, int64_t batch) {
+  const int64_t s = 256 * (d == 128 && ct == 1 ? 3 : 2) / (hkv * nblk);
+  return 3 * batch <= 2 * s ? s : 3 * batch;
+}
 
 }  // namespace
 }  // namespace ftq
@@ -283,13 +289,14 @@ extern "C" int ftq_v1_tree_choose_splits(int batch, int max_query_len, int num_q
   if (batch <= 0 || max_query_len <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 ||
       max_seq_len <= 0)
     return 1;
+  // An even share for each, and three times that when the others are shorter.
   const int64_t ncols = (int64_t)max_query_len * (num_q_heads / num_kv_heads);
-  const int cols = 64 * tree_ct(d, ncols);
-  const int64_t nblk = (ncols + cols - 1) / cols;
-  const int64_t wgs = (int64_t)batch * num_kv_heads * nblk;
-  const int64_t tiles = ((int64_t)max_seq_len + 31) / 32;
-  const int64_t s = std::min<int64_t>(512 / std::max<int64_t>(wgs, 1), tiles / 4);
-  return (int)std::min<int64_t>(std::max<int64_t>(s, 1), 64);
+  const int ct = tree_ct(d, ncols);
+  const int64_t nblk = (ncols + 64 * ct - 1) / (64 * ct);
+  if (nblk * batch * num_kv_heads >= 2048) return 1;  // four rounds of whole sequences
+  const int64_t tiles = ((int64_t)max_seq_len + (d == 64 ? 63 : 31)) / (d == 64 ? 64 : 32);
+  const int64_t s = 3 * tree_parts_all(d, ct, num_kv_heads, nblk, batch) / batch + 1;
+  return (int)std::max<int64_t>(std::min({s, tiles / TREE_PART_MIN, (int64_t)64}), 1);
 }
 
 extern "C" int ftq_v1_tree_attention(const void* query, int q_dtype, int64_t num_tokens, const uint8_t* kv_cache,
@@ -341,9 +348,9 @@ extern "C" int ftq_v1_tree_attention(const void* query, int q_dtype, int64_t num
   a.cache = kv_cache; a.nb = num_blocks; a.sblk = stride_block; a.spos = stride_pos; a.shead = stride_head;
   const int ct = tree_fast_takes(a) ? tree_ct(d, ncols) : tree_ct(d, INT32_MAX);
   const int64_t nblk = (ncols + 64 * ct - 1) / (64 * ct);
+  const int64_t parts = num_splits == 1 ? batch : tree_parts_all(d, ct, num_kv_heads, nblk, batch);
   int64_t grid = 0;
-  FTQ_REQUIRE(!__builtin_mul_overflow(nblk * num_splits, (int64_t)batch * num_kv_heads, &grid) && grid <= INT32_MAX,
-              "tree attention: grid too large");
+  FTQ_REQUIRE(!__builtin_mul_overflow(nblk * num_kv_heads, parts, &grid) && grid <= INT32_MAX, "tree attention: grid too large");
   const bool vrot = (v_flags & V1F_VROT) != 0;
   a.q = query; a.qt = q_dtype; a.tokens = (int)num_tokens;
   while ((1 << a.lbs) < block_size) ++a.lbs;
@@ -361,7 +368,7 @@ extern "C" int ftq_v1_tree_attention(const void* query, int q_dtype, int64_t num
   a.unrot = vrot; a.oscale = vrot ? fwht_scale(d) : 1.f;
   a.lse = lse_out; a.rot = rotation;
   hipStream_t st = (hipStream_t)stream;
-  const hipError_t e = d == 64 ? tree_launch<64>(a, ct, num_tokens, vrot, st) : d == 128 ? tree_launch<128>(a, ct, num_tokens, vrot, st)
-                                                                                    : tree_launch<256>(a, ct, num_tokens, vrot, st);
+  const hipError_t e = d == 64 ? tree_launch<64>(a, ct, (unsigned)grid, num_tokens, vrot, st) : d == 128 ? tree_launch<128>(a, ct, (unsigned)grid, num_tokens, vrot, st)
+                                                                                    : tree_launch<256>(a, ct, (unsigned)grid, num_tokens, vrot, st);
   return hip_status(e);
 }

@@ -243,11 +243,11 @@ __global__ __launch_bounds__(256, D == 128 && CT == 1 ? 3 : 2) void tree_fast_ke
   __shared__ uint32_t table[F::ENTRIES];
   __shared__ int red[4][2];
 
-  const TreeUnit u(a);
   const int G = a.hq / a.hkv, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  if (u.blk * 64 * CT >= u.n * G) return;
-
+  TreeUnit u;
+  TreePart part;
+  if (!tree_share<TK>(a, lane, u, part)) return;
   if constexpr (!F::RAW) {  // pairs of scaled table values
     const float sg = table_scale<1 << KB>(a.cent, true).sigma;
     if (tid < F::ENTRIES)
@@ -259,15 +259,13 @@ __global__ __launch_bounds__(256, D == 128 && CT == 1 ? 3 : 2) void tree_fast_ke
   const int sub = wave * F::TPW / 16, within = wave * F::TPW % 16;
   const uint8_t* head = a.cache + (int64_t)u.kvh * a.shead + (int64_t)within * a.spos;
 
-  for (int blk = u.blk; blk * 64 * CT < u.n * G; blk += a.nblk) {
+  for (; part.blk * 64 * CT < u.n * G; part.blk += a.nblk) {
     W w;
     int first, last;
-    w.columns(a, u, blk, lane, wave, red, u.len, first, last);  // its barrier: the pool is free
-    first = min(first, u.ctx);  // the tree's own positions always
+    w.columns(a, u, part.blk, lane, wave, red, u.len, first, last);  // its barrier: the pool is free
+    first = min(first, u.ctx) / TK;  // the tree's own positions always
     const int held = (int)min((int64_t)u.len, (int64_t)a.max_blocks << a.lbs);  // positions that can have a page
-    const int t0 = first / TK, t1 = max((held + TK - 1) / TK, t0);
-    const int per = (t1 - t0 + a.splits - 1) / a.splits;
-    const int tb0 = t0 + u.split * per, tb1 = min(tb0 + per, t1);
+    const int tb0 = part.part == 0 ? first : max(part.tb0, first), tb1 = min(part.tb1, (held + TK - 1) / TK);
 
     F raw;
     // Block-table entries of the tile to load next, lane k: positions 16 k ..; a
@@ -331,7 +329,7 @@ __global__ __launch_bounds__(256, D == 128 && CT == 1 ? 3 : 2) void tree_fast_ke
     if (CT > 1 && w.nct > 1) run(std::integral_constant<int, CT>{});
     else if (w.nct == 1) run(std::integral_constant<int, 1>{});
     else run(std::integral_constant<int, 0>{});
-    w.finish(a, u, lane);
+    w.finish(a, u, part, lane);
   }
 }
 

@@ -16,8 +16,9 @@
 // more rows of it, 1 / f and (min + mid scale) / f in two parts each: two matrix
 // instructions in place of 32 additions, and the rounding of w is in numerator and
 // denominator alike.
-// The context is split over workgroups where the columns alone do not fill the
-// GPU, and the parts meet in merge_splits_kernel.
+// A sequence's tiles are cut into parts of about one length for all sequences, as
+// many as the GPU holds workgroups (TreeShare): sequences of 1000 and of 6000
+// positions keep them busy alike.  The parts meet in tree_merge_kernel.
 //
 // Operands in LDS, in the order in which lane (m, g) (m = lane & 15, g = lane >> 4)
 // reads its 16 bytes:
@@ -56,7 +57,7 @@ struct TreeArgs {
   const float* cent;
   int kb, vb, flags;
   float qscale;             // of the (unnormalised) rotated query: scale log2 e, and the rotation's norm
-  int splits, nblk;         // grid: column blocks x splits x B x hkv
+  int splits, nblk;         // most parts of a row; 1: a workgroup per column block (nblk a sequence)
   float *wo, *wl;           // partial outputs / log-sum-exps, or
   void* out;                // the output itself (wo == null)
   int ot, unrot;            // its type; whether V is taken back by H
@@ -83,27 +84,111 @@ template <int D> struct TreeGeo {
   __host__ __device__ static constexpr bool vx(int b) { return D != 64 && b >= NB / 2; }
 };
 
-// The sequence, kv head and columns of a workgroup.  Workgroups are dealt to
-// the 8 XCDs in turn; with the kv head fastest, those that read the same slots
-// (the column blocks and splits of one kv head) share an XCD's L2 when there
-// are 8 heads or a multiple.
+// A sequence and kv head.
 struct TreeUnit {
-  int b, kvh, split, blk;
+  int b, kvh;
   int q0, n, ctx, len;      // first query token, query tokens, context positions, all positions
-  __device__ __forceinline__ explicit TreeUnit(const TreeArgs& a) {
-    int id = (int)blockIdx.x;
-    kvh = id % a.hkv;
-    id /= a.hkv;
-    b = id % a.B;
-    id /= a.B;
-    split = id % a.splits;
-    blk = id / a.splits;
+  int t0, t1;               // its tiles: from its first token's start on, to the last position with a page
+  __device__ __forceinline__ void of(const TreeArgs& a, int seq, int tk) {
+    b = seq;
     q0 = min(max(a.qsl[b], 0), a.tokens);
     n = max(min(a.qsl[b + 1], a.tokens) - q0, 0);
     len = max(a.sl[b], n);
     ctx = len - n;
+    const int held = (int)min((int64_t)len, (int64_t)a.max_blocks << a.lbs);
+    t0 = a.ks != nullptr && n > 0 ? min(max(a.ks[q0], 0), ctx) / tk : 0;
+    t1 = max((held + tk - 1) / tk, t0 + 1);
   }
 };
+
+// A workgroup's part of a sequence: tiles [tb0, tb1), of column blocks blk, blk +
+// nblk, ...  Workgroups are dealt to the 8 XCDs in turn; with the kv head fastest and
+// then the block, those that read the same slots at one time share an XCD's L2 when
+// there are 8 heads or a multiple.
+struct TreePart {
+  int blk, tb0, tb1;
+  int part, spare;          // which of the sequence's; spare: those behind it that do not exist, if it is the last (else 0)
+};
+
+// The parts: no longer than a length for which all sequences together have no more
+// parts than there are workgroups (per head and column block; at least one per
+// sequence), found by bisection to 1/16, a lane per sequence.  The tiles of a sequence
+// are dealt evenly to its parts.  False: no part is left for this workgroup.
+constexpr int TREE_PART_MIN = 4;  // tiles
+template <int TK>
+__device__ __forceinline__ bool tree_share(const TreeArgs& a, int lane, TreeUnit& u, TreePart& p) {
+  u.kvh = blockIdx.x % a.hkv;
+  const int id = blockIdx.x / a.hkv, w = id / a.nblk;
+  p.blk = id % a.nblk;
+  if (a.splits == 1) {
+    u.of(a, w, TK);
+    p.tb0 = u.t0; p.tb1 = u.t1; p.part = p.spare = 0;
+    return true;
+  }
+  auto tiles = [&](int b) __attribute__((always_inline)) {
+    if (b >= a.B) return 0;
+    TreeUnit v;
+    v.of(a, b, TK);
+    return v.n > 0 ? v.t1 - v.t0 : 0;
+  };
+  const int mine = tiles(lane);
+  auto total = [&](auto f) __attribute__((always_inline)) {  // f(tiles) over the sequences
+    auto x = f(mine);
+    for (int b0 = 64; b0 < a.B; b0 += 64) x += f(tiles(b0 + lane));
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m);
+    return x;
+  };
+  const int workers = (int)gridDim.x / (a.hkv * a.nblk);  // >= B
+  auto parts = [&](int len) __attribute__((always_inline)) {
+    return __builtin_amdgcn_readfirstlane(total([&](int t) { return (int)((uint32_t)(t + len - 1) / (uint32_t)len); }));
+  };
+  int longest = mine;
+  for (int b0 = 64; b0 < a.B; b0 += 64) longest = max(longest, tiles(b0 + lane));
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) longest = max(longest, __shfl_xor(longest, m));
+  longest = __builtin_amdgcn_readfirstlane(longest);
+  const float sum = total([](int t) { return (float)t; });
+  int lo = max(TREE_PART_MIN, max((longest + a.splits - 1) / a.splits, (int)(sum / (float)workers)));
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  int hi = max(lo, longest);  // at most one part per sequence: fits
+  if (parts(lo) <= workers) {
+    hi = lo;
+  } else {
+    const int guess = __builtin_amdgcn_readfirstlane((int)min(sum / (float)max(workers - a.B, 1) + 2.f, (float)hi));
+    if (guess > lo && guess < hi) {
+      if (parts(guess) <= workers) hi = guess;
+      else lo = guess;
+    }
+    while (hi - lo > 1 + (lo >> 4)) {
+      const int mid = lo + ((hi - lo) >> 1);
+      if (parts(mid) <= workers) hi = mid;
+      else lo = mid;
+    }
+  }
+  for (int b0 = 0, before = 0; b0 < a.B; b0 += 64) {
+    const int own = (int)((uint32_t)((b0 == 0 ? mine : tiles(b0 + lane)) + hi - 1) / (uint32_t)hi);
+    int c = own;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int o = __shfl_up(c, m);
+      if (lane >= m) c += o;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(before + c > w);
+    if (past != 0) {
+      const int l = __builtin_ctzll(past), n = __builtin_amdgcn_readlane(own, l);
+      u.of(a, b0 + l, TK);
+      p.part = w - before - (__builtin_amdgcn_readlane(c, l) - n);
+      const int64_t nt = u.t1 - u.t0;
+      p.tb0 = u.t0 + (int)(nt * p.part / n);
+      p.tb1 = u.t0 + (int)(nt * (p.part + 1) / n);
+      p.spare = p.part == n - 1 ? a.splits - n : 0;
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(c, 63);
+  }
+  return false;
+}
 
 // What the sequence's token r attends of the 32 positions from pos0 on: the context
 // from its start on, and the tokens of its mask (null: those up to its own).
@@ -497,7 +582,7 @@ struct TreeWave {
   }
 
   // Lane (n, g) holds dims NB (4 g + i) + b of column n.
-  __device__ __forceinline__ void finish(const TreeArgs& a, const TreeUnit& u, int lane) {
+  __device__ __forceinline__ void finish(const TreeArgs& a, const TreeUnit& u, const TreePart& part, int lane) {
     const int n = lane & 15, g = lane >> 4, G = a.hq / a.hkv;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
@@ -514,10 +599,13 @@ struct TreeWave {
       const int64_t at = (int64_t)(u.q0 + row[ct]) * a.hq + u.kvh * G + (c0 + 16 * ct + n - row[ct] * G);
       if (a.wo != nullptr) {
         if (row[ct] >= 0) {
-          const int64_t r = at * a.splits + u.split;
+          const int64_t r = at * a.splits + part.part;
 #pragma unroll
           for (int i = 0; i < 4; ++i) store_elems<F32, NB>(a.wo, r * D + NB * (4 * g + i), y[i]);
-          if (g == 0) a.wl[r] = none ? -INFINITY : m_run[ct] + __builtin_log2f(L * (1.f / TREE_LIFT));
+          if (g == 0) {
+            a.wl[r] = none ? -INFINITY : m_run[ct] + __builtin_log2f(L * (1.f / TREE_LIFT));
+            for (int k = 1; k <= part.spare; ++k) a.wl[r + k] = -INFINITY;
+          }
         }
         continue;
       }
@@ -554,5 +642,80 @@ struct TreeWave {
     }
   }
 };
+
+// Partial outputs of a row -> the row: the parts' log-sum-exps (log2 domain), -inf
+// behind the last, weigh them; then the output transform, MergeRot of ftq_merge.h.
+// A wave per row; rows behind the last sequence stay as they are.
+template <int D, int OT, int ROT>
+__global__ __launch_bounds__(256) void tree_merge_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_lse,
+                                                         const int32_t* __restrict__ tokens_end, int tokens, int hq, int splits,
+                                                         const float* __restrict__ rot, float scale, void* __restrict__ out,
+                                                         float* __restrict__ lse_out) {
+  constexpr int E = D / 64;
+  __shared__ float mrow[ROT == ROT_MATRIX ? 4 : 1][ROT == ROT_MATRIX ? D : 1];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int64_t r = (int64_t)blockIdx.x * 4 + wv;
+  if (r >= (int64_t)min(max(*tokens_end, 0), tokens) * hq) return;
+  const float* lse = ws_lse + r * splits;
+  float M = -INFINITY;
+  bool nan = false;
+  int np = 0;  // parts to add
+  for (int s0 = 0; s0 < splits; s0 += 64) {
+    const float l = s0 + lane < splits ? lse[s0 + lane] : -INFINITY;
+    M = fmaxf(M, l);
+    nan = nan || l != l;
+    const uint64_t some = __builtin_amdgcn_ballot_w64(l > -INFINITY);
+    if (some != 0) np = s0 + 64 - __builtin_clzll(some);
+  }
+  M = wave_max64(M);
+  nan = __builtin_amdgcn_ballot_w64(nan) != 0;  // the maximum does not show it
+  float y[E], W = 0.f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) y[i] = 0.f;
+  const float* po = ws_o + r * splits * D + lane * E;
+  constexpr int CH = 8;
+  for (int s0 = 0; s0 < np; s0 += CH) {
+    float x[CH][E], l[CH];
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+      if (s0 + k < np) {
+        load_f32_small<E>(po + (int64_t)(s0 + k) * D, x[k]);
+        l[k] = lse[s0 + k];
+      }
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+      if (s0 + k < np) {
+        const float w = __builtin_amdgcn_exp2f(l[k] - M);
+        W += w;
+#pragma unroll
+        for (int i = 0; i < E; ++i) y[i] = __builtin_fmaf(w, x[k][i], y[i]);
+      }
+  }
+  if (nan) W = __builtin_nanf("");
+  if (lse_out != nullptr && lane == 0) lse_out[r] = W == 0.f ? -INFINITY : (M + __builtin_log2f(W)) * 0.69314718055994531f;
+  const float inv = W == 0.f ? 0.f : 1.f / W;
+#pragma unroll
+  for (int i = 0; i < E; ++i) y[i] *= inv;
+  if constexpr (ROT == ROT_MATRIX) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) mrow[wv][lane * E + i] = y[i];
+    __asm__ volatile("" ::: "memory");  // this wave's row; a wave's LDS accesses run in order
+    float z[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) z[i] = 0.f;
+    for (int j = 0; j < D; ++j) {
+      const float oj = mrow[wv][j];
+#pragma unroll
+      for (int i = 0; i < E; ++i) z[i] = __builtin_fmaf(oj, rot[(int64_t)(lane * E + i) * D + j], z[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) y[i] = z[i];
+  } else if constexpr (ROT == ROT_PLAIN) {
+    fwht_wave64<E>(y, lane);
+#pragma unroll
+    for (int i = 0; i < E; ++i) y[i] *= scale;
+  }
+  store_small<OT, E>(out, r * D + lane * E, y);
+}
 
 }  // namespace ftq

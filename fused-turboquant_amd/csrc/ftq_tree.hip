@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   TreeUnit u;
   TreePart part;
-  if (!tree_share<TK>(a, lane, u, part)) return;
+  if (!tree_share<TK>(a, TreeMine(a, lane), lane, u, part)) return;
   const bool raw = a.kb == TREE_RAW, kf8 = (a.flags & V1F_KFP8) != 0;
   const V1Geom geo = raw ? V1Geom{2 * D, 2 * D, 2 * D, 4 * D} : v1_geom(D, a.kb, a.vb, kf8);
   const int nd = (geo.raw + 3) / 4, pitch = (nd + 1) | 1;
@@ -97,7 +97,9 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
     W w;
     int first, last;
     w.columns(a, u, part.blk, lane, wave, red, u.len, first, last);  // its barrier: the pool is free, and the tables written
-    w.queries(a, u, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
+    typename W::Raw q;
+    w.fetch(a, u, lane, q);
+    w.queries(a, u, q, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
     __syncthreads();
     first = min(first, u.ctx) / TK;  // the tree's own positions always
     const int tb0 = part.part == 0 ? first : max(part.tb0, first), tb1 = part.tb1;
@@ -271,10 +273,10 @@ hipError_t tree_launch(const TreeArgs& a, int ct, unsigned grid, int64_t tokens,
 // columns do (fewer registers, more workgroups a CU).
 int tree_ct(int d, int64_t cols) { return d == 256 || cols <= 64 ? 1 : 2; }
 // Parts (TreeShare) of all sequences together, per kv head and column block: what the
-// 256 CUs hold at once (three workgroups a CU at d = 128 with one column tile a wave,
-// else two); where that is hardly more than the sequences, three rounds of it or more.
+// 256 CUs hold at once (three workgroups a CU with one column tile a wave below
+// d = 256, else two); where that is hardly more than the sequences, three rounds of it or more.
 int64_t tree_parts_all(int d, int ct, int hkv, int64_t nblk, int64_t batch) {
-  const int64_t s = 256 * (d == 128 && ct == 1 ? 3 : 2) / (hkv * nblk);
+  const int64_t s = 256 * (d != 256 && ct == 1 ? 3 : 2) / (hkv * nblk);
   return 3 * batch <= 2 * s ? s : 3 * batch;
 }
 

@@ -232,7 +232,7 @@ struct TreeFmt {
 };
 
 template <int D, int KB, int VB, int NH, int CT>
-__global__ __launch_bounds__(256, D == 128 && CT == 1 ? 3 : 2) void tree_fast_kernel(const TreeArgs a) {
+__global__ __launch_bounds__(256, D <= 128 && CT == 1 ? 3 : 2) void tree_fast_kernel(const TreeArgs a) {
   using C = TreeGeo<D>;
   using F = TreeFmt<D, KB, VB>;
   constexpr int TK = C::TK, NT = C::NT, NP = C::NP;
@@ -245,14 +245,15 @@ __global__ __launch_bounds__(256, D == 128 && CT == 1 ? 3 : 2) void tree_fast_ke
 
   const int G = a.hq / a.hkv, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  TreeUnit u;
-  TreePart part;
-  if (!tree_share<TK>(a, lane, u, part)) return;
+  const TreeMine mine(a, lane);
   if constexpr (!F::RAW) {  // pairs of scaled table values
     const float sg = table_scale<1 << KB>(a.cent, true).sigma;
     if (tid < F::ENTRIES)
       table[tid] = f32_to_f16_bits(sg * a.cent[tid & ((1 << KB) - 1)]) | f32_to_f16_bits(sg * a.cent[tid >> KB]) << 16;
   }
+  TreeUnit u;
+  TreePart part;
+  if (!tree_share<TK>(a, mine, lane, u, part)) return;
   const uint32_t s_pos = (uint32_t)a.spos;
   const int nb32 = (int)min(a.nb, (int64_t)0x7fffffff);
   // the wave's positions of a tile lie in one run of 16
@@ -286,11 +287,12 @@ __global__ __launch_bounds__(256, D == 128 && CT == 1 ? 3 : 2) void tree_fast_ke
       entries(min(t + 1, tb1 - 1));
     };
     uint32_t now = 0;  // `on` of the tile that is multiplied
-    if (tb0 < tb1) {  // the first bytes are on their way while the queries are rotated
-      entries(tb0);
-      fetch(tb0);
-    }
-    w.queries(a, u, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
+    // the queries and the first bytes are on their way together
+    typename W::Raw q;
+    if (tb0 < tb1) entries(tb0);
+    w.fetch(a, u, lane, q);
+    if (tb0 < tb1) fetch(tb0);
+    w.queries(a, u, q, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
     __syncthreads();
     if (tid < 2 * 64 * NP) pool[tid / (64 * NP) * B::SIZE + B::X + tid % (64 * NP)] = u32x4{0, 0, 0, 0};
     __syncthreads();

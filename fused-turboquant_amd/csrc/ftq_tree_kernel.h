@@ -89,11 +89,12 @@ struct TreeUnit {
   int b, kvh;
   int q0, n, ctx, len;      // first query token, query tokens, context positions, all positions
   int t0, t1;               // its tiles: from its first token's start on, to the last position with a page
-  __device__ __forceinline__ void of(const TreeArgs& a, int seq, int tk) {
+  __device__ __forceinline__ void of(const TreeArgs& a, int seq, int tk) { of(a, seq, a.qsl[seq], a.qsl[seq + 1], a.sl[seq], tk); }
+  __device__ __forceinline__ void of(const TreeArgs& a, int seq, int begin, int end, int positions, int tk) {
     b = seq;
-    q0 = min(max(a.qsl[b], 0), a.tokens);
-    n = max(min(a.qsl[b + 1], a.tokens) - q0, 0);
-    len = max(a.sl[b], n);
+    q0 = min(max(begin, 0), a.tokens);
+    n = max(min(end, a.tokens) - q0, 0);
+    len = max(positions, n);
     ctx = len - n;
     const int held = (int)min((int64_t)len, (int64_t)a.max_blocks << a.lbs);
     t0 = a.ks != nullptr && n > 0 ? min(max(a.ks[q0], 0), ctx) / tk : 0;
@@ -115,8 +116,19 @@ struct TreePart {
 // sequence), found by bisection to 1/16, a lane per sequence.  The tiles of a sequence
 // are dealt evenly to its parts.  False: no part is left for this workgroup.
 constexpr int TREE_PART_MIN = 4;  // tiles
+// What the lane's sequence is read from; apart from tree_share, so that other work can
+// be done meanwhile.
+struct TreeMine {
+  int begin, end, positions;
+  __device__ __forceinline__ TreeMine(const TreeArgs& a, int lane) {
+    const int b = min(lane, a.B - 1);
+    begin = a.qsl[b];
+    end = a.qsl[b + 1];
+    positions = a.sl[b];
+  }
+};
 template <int TK>
-__device__ __forceinline__ bool tree_share(const TreeArgs& a, int lane, TreeUnit& u, TreePart& p) {
+__device__ __forceinline__ bool tree_share(const TreeArgs& a, const TreeMine& m, int lane, TreeUnit& u, TreePart& p) {
   u.kvh = blockIdx.x % a.hkv;
   const int id = blockIdx.x / a.hkv, w = id / a.nblk;
   p.blk = id % a.nblk;
@@ -131,7 +143,9 @@ __device__ __forceinline__ bool tree_share(const TreeArgs& a, int lane, TreeUnit
     v.of(a, b, TK);
     return v.n > 0 ? v.t1 - v.t0 : 0;
   };
-  const int mine = tiles(lane);
+  TreeUnit v;
+  v.of(a, min(lane, a.B - 1), m.begin, m.end, m.positions, TK);
+  const int mine = lane < a.B && v.n > 0 ? v.t1 - v.t0 : 0;
   auto total = [&](auto f) __attribute__((always_inline)) {  // f(tiles) over the sequences
     auto x = f(mine);
     for (int b0 = 64; b0 < a.B; b0 += 64) x += f(tiles(b0 + lane));
@@ -179,9 +193,9 @@ __device__ __forceinline__ bool tree_share(const TreeArgs& a, int lane, TreeUnit
       const int l = __builtin_ctzll(past), n = __builtin_amdgcn_readlane(own, l);
       u.of(a, b0 + l, TK);
       p.part = w - before - (__builtin_amdgcn_readlane(c, l) - n);
-      const int64_t nt = u.t1 - u.t0;
-      p.tb0 = u.t0 + (int)(nt * p.part / n);
-      p.tb1 = u.t0 + (int)(nt * (p.part + 1) / n);
+      const uint32_t nt = u.t1 - u.t0, each = nt / (uint32_t)n, more = nt - each * n;  // the first parts: one more
+      p.tb0 = u.t0 + (int)(p.part * each + min((uint32_t)p.part, more));
+      p.tb1 = p.tb0 + (int)(each + ((uint32_t)p.part < more ? 1u : 0u));
       p.spare = p.part == n - 1 ? a.splits - n : 0;
       return true;
     }
@@ -331,57 +345,73 @@ struct TreeWave {
     last = __builtin_amdgcn_readfirstlane(max(max(red[0][1], red[1][1]), max(red[2][1], red[3][1])));
   }
 
-  // The columns' queries, rotated and scaled, as f16 hi + lo.  One query per 16
-  // lanes, four at a time, through 16 rows of LDS of the wave's own.
-  __device__ __forceinline__ void queries(const TreeArgs& a, const TreeUnit& u, int lane, float (*rows)[D + 4]) {
-    constexpr int E = D / 16;
-    const int G = a.hq / a.hkv, l16 = lane & 15, g = lane >> 4, n = lane & 15;
+  // The columns' queries as they are stored; four lanes per query
+  struct Raw {
+    static constexpr int E = D / 4;
+    u32x4 x[CT][E / 4];
+  };
+  __device__ __forceinline__ void fetch(const TreeArgs& a, const TreeUnit& u, int lane, Raw& q) {
+    constexpr int E = Raw::E;
+    const int G = a.hq / a.hkv;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int col = min(c0 + 16 * ct + (lane >> 2), u.n * G - 1);  // behind the last: it again, for nobody
+      const int r = col / G, h = u.kvh * G + (col - r * G);
+      const int64_t off = ((int64_t)(u.q0 + r) * a.hq + h) * D + (lane & 3) * E;
+      const u32x4* src = reinterpret_cast<const u32x4*>(static_cast<const char*>(a.q) + off * (a.qt == F32 ? 4 : 2));
+#pragma unroll
+      for (int i = 0; i < E / 8; ++i) q.x[ct][i] = src[i];
+#pragma unroll
+      for (int i = E / 8; i < E / 4; ++i) q.x[ct][i] = a.qt == F32 ? src[i] : u32x4{0, 0, 0, 0};
+    }
+  }
+
+  // The columns' queries, rotated and scaled, as f16 hi + lo, through 16 rows of LDS
+  // of the wave's own.  Four lanes per query: most butterflies of the transform stay
+  // inside a lane.
+  __device__ __forceinline__ void queries(const TreeArgs& a, const TreeUnit& u, const Raw& q, int lane, float (*rows)[D + 4]) {
+    constexpr int E = D / 4;
+    const int l4 = lane & 3, mine = lane >> 2, g = lane >> 4, n = lane & 15;
     qlarge = 0;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       float inv = 1.f;
       if (ct < nct) {
-        float y[4][E];  // all four loads at once
+        float y[E];
+        const bool on = c0 + 16 * ct + mine < u.n * (a.hq / a.hkv);
+        if (a.qt == F32) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int col = c0 + 16 * ct + 4 * k + g;
-          const bool on = col < u.n * G;
-          const int r = on ? col / G : 0, h = u.kvh * G + (on ? col - r * G : 0);
-          const int64_t off = ((int64_t)(u.q0 + r) * a.hq + h) * D + l16 * E;
-          if (a.qt == F32) load_elems<F32, E>(a.q, off, y[k]);
-          else if (a.qt == F16) load_elems<F16, E>(a.q, off, y[k]);
-          else load_elems<BF16, E>(a.q, off, y[k]);
-#pragma unroll
-          for (int i = 0; i < E; ++i) y[k][i] = on ? y[k][i] : 0.f;
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (a.kb != TREE_RAW) {
-            if (a.rot != nullptr) rot_matrix_lanes<D, E>(y[k], a.rot, rows[4 * k + g], l16);
-            else fwht_lanes<E, 16>(y[k], l16);
-          }
-          float mx = 0.f;
+          for (int i = 0; i < E; ++i) y[i] = __uint_as_float(q.x[ct][i >> 2][i & 3]);
+        } else {
 #pragma unroll
           for (int i = 0; i < E; ++i) {
-            y[k][i] *= a.qscale;
-            mx = fmaxf(mx, fabsf(y[k][i]));
+            const uint32_t w = q.x[ct][i >> 3][(i >> 1) & 3];
+            y[i] = half_bits_to_f32(a.qt == F16 ? F16 : BF16, i & 1 ? w >> 16 : w & 0xffffu);
           }
-          mx = fmaxf(mx, lane_xor<1>(mx));
-          mx = fmaxf(mx, lane_xor<2>(mx));
-          mx = fmaxf(mx, lane_xor<4>(mx));
-          mx = fmaxf(mx, lane_xor<8>(mx));
-          // A query that f16 cannot hold is scaled to [2^13, 2^14).  Small ones need
-          // no scale: what their low parts lose below f16's range is 2^-25 of a
-          // score, an absolute error.
-          const int e = (int)((__float_as_uint(mx) >> 23) & 255u);
-          const int ue = e >= 127 + 14 && e < 255 ? 140 + 127 - e : 127;
-          const float up = __uint_as_float((uint32_t)ue << 23);
-          const float down = __uint_as_float((uint32_t)(254 - ue) << 23);
-          const float got = __shfl(down, (n & 3) << 4);  // of column 4 k + (n & 3)
-          if ((n >> 2) == k) inv = got;
-#pragma unroll
-          for (int i = 0; i < E; ++i) rows[4 * k + g][l16 * E + i] = y[k][i] * up;
         }
+#pragma unroll
+        for (int i = 0; i < E; ++i) y[i] = on ? y[i] : 0.f;
+        if (a.kb != TREE_RAW) {
+          if (a.rot != nullptr) rot_matrix_lanes<D, E>(y, a.rot, rows[mine], l4);
+          else fwht_lanes<E, 4>(y, l4);
+        }
+        float mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          y[i] *= a.qscale;
+          mx = fmaxf(mx, fabsf(y[i]));
+        }
+        mx = fmaxf(mx, lane_xor<1>(mx));
+        mx = fmaxf(mx, lane_xor<2>(mx));
+        // A query that f16 cannot hold is scaled to [2^13, 2^14).  Small ones need
+        // no scale: what their low parts lose below f16's range is 2^-25 of a
+        // score, an absolute error.
+        const int e = (int)((__float_as_uint(mx) >> 23) & 255u);
+        const int ue = e >= 127 + 14 && e < 255 ? 140 + 127 - e : 127;
+        const float up = __uint_as_float((uint32_t)ue << 23);
+        inv = __shfl(__uint_as_float((uint32_t)(254 - ue) << 23), n << 2);  // column n's
+#pragma unroll
+        for (int i = 0; i < E; ++i) rows[mine][l4 * E + i] = y[i] * up;
         __asm__ volatile("" ::: "memory");  // a wave's LDS accesses run in order
       }
 #pragma unroll

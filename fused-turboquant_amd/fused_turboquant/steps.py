@@ -153,16 +153,22 @@ def commit_slots(kv_caches: Sequence[torch.Tensor], block_table: torch.Tensor, p
     pth = _ints("path", path, 2)
     if past.numel() != B or cnt.numel() != B or pth.shape[0] != B:
         raise ValueError("past_lens, counts and path must have one entry (row) per row of block_table")
-    for c in caches:
-        if c.dtype != torch.uint8 or c.dim() != 4:
-            raise ValueError("kv_caches must be uint8 [num_blocks, block_size, num_kv_heads, slot]")
-        if c.shape != caches[0].shape or c.stride() != caches[0].stride():
-            raise ValueError("kv_caches must have one shape and layout")
-        if c.stride(3) != 1:
-            raise ValueError("kv_cache slot bytes must be contiguous")
-    if len({c.data_ptr() for c in caches}) != len(caches):
-        raise ValueError("kv_caches names a cache twice")
     if not caches:
         return
-    _lib.require_device(*caches, block_table, past, pth, cnt)
+    first = caches[0]
+    if first.dim() != 4:
+        raise ValueError("kv_caches must be uint8 [num_blocks, block_size, num_kv_heads, slot]")
+    shape, stride, device = first.shape, first.stride(), first.device
+    if stride[3] != 1:
+        raise ValueError("kv_cache slot bytes must be contiguous")
+    seen = set()
+    for c in caches:  # (once per layer and step: few calls each)
+        if c.dtype != torch.uint8:
+            raise ValueError("kv_caches must be uint8 [num_blocks, block_size, num_kv_heads, slot]")
+        if c.shape != shape or c.stride() != stride or c.device != device:
+            raise ValueError("kv_caches must have one shape and layout, on one device")
+        seen.add(c.data_ptr())
+    if len(seen) != len(caches):
+        raise ValueError("kv_caches names a cache twice")
+    _lib.require_device(first, block_table, past, pth, cnt)
     _ops.ops().commit_slots(caches, block_table.contiguous(), past, pth, cnt)

@@ -5,6 +5,7 @@ launch on the device where a host program would synchronise:
   tokens from the requests' lengths; with a free list, the pages a request
   gains or gives back.
 * ``tree_accept``: the accepted path of every drafted tree.
+* ``tree_shape``: depths and mask of a tree (on the host).
 * ``commit_slots``: the accepted tokens' slots moved to consecutive positions,
   in every layer's cache.
 
@@ -21,6 +22,9 @@ from typing import NamedTuple, Optional, Sequence
 import torch
 
 from . import _lib, _ops
+
+
+MAX_REQUESTS = 4096  # of one step_tables call
 
 
 class StepTables(NamedTuple):
@@ -49,6 +53,28 @@ def _in_place(name: str, t: torch.Tensor) -> torch.Tensor:
     if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of one dimension")
     return t
+
+
+def tree_shape(parents: Sequence[int]) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(depths, mask)`` of a tree from its nodes' parents (the root's -1
+    first, every parent before its children): int32 [n], and int64 [n, words]
+    with bit j of a node's row set for its ancestors and itself, the
+    ``tree_mask`` of ``v1.v1_tree_attention``.  Host tensors, computed once
+    for a tree that is drafted again and again."""
+    n = len(parents)
+    if n == 0 or parents[0] != -1:
+        raise ValueError("parents must start with the root's -1")
+    depth, rows = [0], [1]
+    for i in range(1, n):
+        p = int(parents[i])
+        if not 0 <= p < i:
+            raise ValueError(f"parents[{i}] = {p}: a parent comes before its children, and there is one root")
+        depth.append(depth[p] + 1)
+        rows.append(rows[p] | 1 << i)
+    low = (1 << 64) - 1
+    words = [[(r >> 64 * w) & low for w in range((n + 63) // 64)] for r in rows]
+    signed = [[x - (1 << 64) if x >> 63 else x for x in r] for r in words]
+    return torch.tensor(depth, dtype=torch.int32), torch.tensor(signed, dtype=torch.int64)
 
 
 def step_tables(query_start_loc: torch.Tensor, past_lens: torch.Tensor, block_table: torch.Tensor, block_size: int,
@@ -80,8 +106,8 @@ def step_tables(query_start_loc: torch.Tensor, past_lens: torch.Tensor, block_ta
     B = past.numel()
     if qsl.numel() != B + 1:
         raise ValueError("query_start_loc must have one entry more than past_lens")
-    if B > 4096:
-        raise ValueError("step_tables takes at most 4096 requests")
+    if B > MAX_REQUESTS:
+        raise ValueError(f"step_tables takes at most {MAX_REQUESTS} requests")
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError("block_table must be int32 [B, max_blocks]")
     if block_table.numel() and block_table.shape[1] > 1 and block_table.stride(1) != 1 or (B > 1 and block_table.stride(0) < block_table.shape[1]):

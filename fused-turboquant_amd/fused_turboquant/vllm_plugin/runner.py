@@ -28,7 +28,11 @@ exactly as vLLM's ``Attention`` layer calls them):
   (``max_num_batched_tokens``), greedy sampling, and decode steps captured
   once in a HIP graph and replayed (vLLM's CUDA-graph mode), with the step's
   positions, slots and sequence lengths computed on the device inside the
-  graph.
+  graph (``steps.step_tables``).  ``generate_tree`` decodes with trees of
+  drafted tokens (speculative decoding): one step stores every node, attends
+  through ``v1.v1_tree_attention``, takes the target's token after each node,
+  walks the accepted path (``steps.tree_accept``) and moves its slots together
+  (``steps.commit_slots``); the result is the model's own greedy decode.
 
 The attention of each layer is either the ``TURBOQUANT`` Impl or
 ``DenseAttention``, a plain bf16 paged cache with torch SDPA, the baseline
@@ -44,6 +48,7 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 
+from .. import steps as STEPS
 from .v1_backend import FusedTurboQuantV1Backend, FusedTurboQuantV1Impl
 
 
@@ -76,6 +81,8 @@ class StepMetadata:
     max_query_len: int
     max_seq_len: int
     slot_mapping: torch.Tensor     # int64 [num_tokens]
+    tree_mask: Optional[torch.Tensor] = None        # int64 [num_tokens, words]: a step of drafted trees
+    token_positions: Optional[torch.Tensor] = None  # int64 [num_tokens], for trees on sliding-window layers
 
 
 class BlockAllocator:
@@ -326,8 +333,12 @@ class ModelRunner:
         st = self._st
         bs = self.block_size
         pos = st.pos
-        seq_lens = (pos + 1).to(torch.int32)
-        slots = st.bt.gather(1, (pos // bs)[:, None]).squeeze(1).long() * bs + pos % bs
+        if self.device.type == "cuda" and st.B <= STEPS.MAX_REQUESTS:
+            t = STEPS.step_tables(st.qsl, pos.to(torch.int32), st.bt, bs, st.B)
+            seq_lens, slots = t.seq_lens, t.slot_mapping
+        else:
+            seq_lens = (pos + 1).to(torch.int32)
+            slots = st.bt.gather(1, (pos // bs)[:, None]).squeeze(1).long() * bs + pos % bs
         md = StepMetadata(num_actual_tokens=st.B, is_prefill=False, num_decodes=st.B, num_decode_tokens=st.B,
                           seq_lens=seq_lens, block_table=st.bt, query_start_loc=st.qsl, max_query_len=1,
                           max_seq_len=st.max_seq_len, slot_mapping=slots)
@@ -357,25 +368,26 @@ class ModelRunner:
             out=torch.zeros(max_steps, B, dtype=torch.int64, device=dev),
             step=torch.zeros(1, dtype=torch.int64, device=dev),
             max_seq_len=max(prompt_lens) + max_steps)
-        self.graph = None
-        if use_graph:
-            st = self._st
-            saved = (st.tok.clone(), st.pos.clone(), st.out.clone(), st.step.clone())
-            side = torch.cuda.Stream(device=dev)
-            side.wait_stream(torch.cuda.current_stream(dev))
-            with torch.cuda.stream(side):
-                self._decode_body()  # allocates the per-layer scratch outside the capture
-            torch.cuda.current_stream(dev).wait_stream(side)
-            torch.cuda.synchronize(dev)
-            st.tok.copy_(saved[0])
-            st.pos.copy_(saved[1])
-            st.out.copy_(saved[2])
-            st.step.copy_(saved[3])
-            g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g):
-                self._decode_body()
-            # the capture recorded the step without running it: state is still the start
-            self.graph = g
+        st = self._st
+        self.graph = self._capture(self._decode_body, (st.tok, st.pos, st.out, st.step)) if use_graph else None
+
+    def _capture(self, body, state):
+        """``body`` in a HIP graph, after a run of it on a side stream that
+        allocates the per-layer scratch; ``state`` is put back afterwards."""
+        dev = self.device
+        saved = [t.clone() for t in state]
+        side = torch.cuda.Stream(device=dev)
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(side):
+            body()
+        torch.cuda.current_stream(dev).wait_stream(side)
+        torch.cuda.synchronize(dev)
+        for t, v in zip(state, saved):
+            t.copy_(v)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            body()
+        return g  # the capture recorded the step without running it: state is still the start
 
     def decode_step(self, force: Optional[torch.Tensor] = None):
         """One decode step of every request; ``force`` (int64 [B]) replaces
@@ -400,3 +412,97 @@ class ModelRunner:
         for _ in range(steps):
             self.decode_step()
         return torch.cat([first[:, None], self._st.out[:steps].t()], dim=1)
+
+    # -- decode with trees of drafted tokens ----------------------------------
+    def _tree_body(self):
+        st = self._st
+        B, n = st.nodes.shape
+        nodes = st.nodes.view(-1)
+        st.nodes[:, 0].copy_(st.tok)
+        t = STEPS.step_tables(st.qsl, st.past, st.bt, self.block_size, B * n, depths=st.depths)
+        md = StepMetadata(num_actual_tokens=B * n, is_prefill=False, num_decodes=B, num_decode_tokens=B * n,
+                          seq_lens=t.seq_lens, block_table=st.bt, query_start_loc=st.qsl, max_query_len=n,
+                          max_seq_len=st.max_seq_len, slot_mapping=t.slot_mapping, tree_mask=st.mask,
+                          token_positions=t.positions)
+        capturing = torch.cuda.is_current_stream_capturing()
+        logits = self.model.forward(nodes, t.positions, md, self.attn, self.layer_objs, self.kv_caches, st.rows,
+                                    attn_hook=None if capturing else self.attn_hook)
+        if self.keep_logits and not capturing:
+            self.logits.append(logits)
+        got = STEPS.tree_accept(nodes, st.parents, logits.argmax(dim=-1), st.qsl, n)
+        # no more than the request still wants: its last tokens, then nothing
+        counts = torch.minimum(got.counts, st.most - st.lens)
+        STEPS.commit_slots(self.kv_caches, st.bt, st.past, got.path, counts)
+        # behind the accepted ones: into the column that nobody reads
+        at = torch.where(st.cols < counts[:, None], st.lens[:, None] + st.cols, st.most)
+        st.out.scatter_(1, at.long(), got.tokens)
+        last = got.tokens.gather(1, (counts - 1).clamp_(min=0).long()[:, None]).squeeze(1)
+        st.tok.copy_(torch.where(counts > 0, last, st.tok))
+        st.past.add_(counts)
+        st.lens.add_(counts)
+
+    def start_tree(self, block_table: torch.Tensor, first_tokens: torch.Tensor, prompt_lens: list[int],
+                   max_tokens: int, parents: list[int], use_graph: bool = True):
+        """Device state of a decode run with trees of drafted tokens, of one
+        shape for all requests and steps: ``parents`` of its nodes (the root's
+        -1 first; the root is the last sampled token).  Up to ``max_tokens``
+        tokens per request; with ``use_graph`` a step is captured in a HIP
+        graph."""
+        if self.backend != "turboquant":
+            raise NotImplementedError("trees of drafted tokens need backend='turboquant'")
+        dev, bs = self.device, self.block_size
+        B, n = first_tokens.shape[0], len(parents)
+        depths, mask = STEPS.tree_shape(parents)
+        longest = max(prompt_lens) + max_tokens + n  # a step's nodes behind the accepted tokens
+        if max_tokens < 1 or longest > block_table.shape[1] * bs or longest > self.model.spec.max_positions:
+            raise ValueError(f"{max(prompt_lens)} + {max_tokens} tokens and a tree of {n} exceed the context")
+        self._st = SimpleNamespace(
+            bt=block_table, tok=first_tokens.clone(), rows=torch.arange(B * n, device=dev),
+            cols=torch.arange(n, dtype=torch.int32, device=dev),
+            past=torch.tensor(prompt_lens, dtype=torch.int32, device=dev), max_seq_len=longest,
+            lens=torch.zeros(B, dtype=torch.int32, device=dev), most=max_tokens,
+            out=torch.zeros(B, max_tokens + 1, dtype=torch.int64, device=dev),
+            qsl=torch.arange(B + 1, dtype=torch.int32, device=dev) * n,
+            nodes=torch.zeros(B, n, dtype=torch.int64, device=dev),
+            parents=torch.tensor(parents, dtype=torch.int32, device=dev).repeat(B),
+            depths=depths.to(dev).repeat(B), mask=mask.to(dev).repeat(B, 1))
+        st = self._st
+        self.graph = self._capture(self._tree_body, (st.tok, st.past, st.lens, st.out)) if use_graph else None
+
+    def tree_step(self, drafted: torch.Tensor):
+        """One step: ``drafted`` (int64 [B, n - 1]) are the tokens of the nodes
+        behind the root.  Each request gains one token or more, until it has
+        its ``max_tokens``."""
+        st = self._st
+        if tuple(drafted.shape) != (st.nodes.shape[0], st.nodes.shape[1] - 1):
+            raise ValueError(f"drafted must be [{st.nodes.shape[0]}, {st.nodes.shape[1] - 1}]")
+        st.nodes[:, 1:].copy_(drafted)
+        if self.graph is not None:
+            self.graph.replay()
+        else:
+            self._tree_body()
+
+    def tree_tokens(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """The decoded tokens so far, int64 [B, max_tokens], and how many of
+        each row there are, int32 [B]."""
+        return self._st.out[:, :self._st.most], self._st.lens
+
+    def generate_tree(self, prompts: list[torch.Tensor], max_new_tokens: int, parents: list[int], draft,
+                      use_graph: bool = True) -> torch.Tensor:
+        """Greedy generation with drafted trees, [B, max_new_tokens] int64.
+        ``draft(tokens, lens)`` proposes the nodes behind the root, int64 [B,
+        len(parents) - 1], from the requests' new tokens so far (int64 [B,
+        max_new_tokens]; ``lens`` int32 [B] of each row are there)."""
+        bt, first = self.prefill(prompts)
+        done = torch.zeros(len(prompts), max_new_tokens, dtype=torch.int64, device=self.device)
+        done[:, 0] = first
+        if max_new_tokens == 1:
+            return done
+        self.start_tree(bt, first, [int(p.numel()) for p in prompts], max_new_tokens - 1, parents, use_graph=use_graph)
+        lens = torch.ones(len(prompts), dtype=torch.int32, device=self.device)
+        while int(lens.min()) < max_new_tokens:  # (the host reads the lengths to stop)
+            self.tree_step(draft(done, lens))
+            tokens, got = self.tree_tokens()
+            done[:, 1:].copy_(tokens)
+            lens = got + 1
+        return done

@@ -41,6 +41,15 @@ query block to its window.  The reference stores the window and attends the
 whole context (``:316``); logit soft-capping, which it also stores without
 applying (``:318``), is refused here.
 
+Trees of drafted tokens (speculative decoding): a decode step whose metadata
+has a ``tree_mask`` (int64 [num_actual_tokens, words], bit j of a token's row:
+it attends token j of its request) gives each request the tokens
+``query_start_loc`` names instead of one, and runs ``ftq_v1_tree_attention``
+over every slot format, raw boundary layers included.  A sliding-window layer
+also needs ``token_positions`` (int64 or int32 [num_actual_tokens], the depth
+in the tree counted) and no tree larger than its window.  Deferred prefill is
+refused.  The reference decodes one token a request.
+
 Head sizes 64, 128 and 256.  With 2-4 bit codes decode runs on the
 matrix-core kernels (64 and 256 at float32-level products); the other widths
 (1-bit, 8-bit, fp8 keys) run the fp32 decode kernel.
@@ -367,11 +376,16 @@ class FusedTurboQuantV1Impl(_ImplBase):
             # decode-only step: straight into vLLM's output buffer, per-layer
             # scratch, no host reads -- capturable in a CUDA/HIP graph
             o3 = output[:N].view(N, self.num_heads, self.head_size)
+            if getattr(attn_metadata, "tree_mask", None) is not None:
+                self._tree(q, kv_cache, attn_metadata, st, layer, o3)
+                return output
             if output.dtype == query.dtype and o3.is_contiguous():
                 dec = self._decode_hybrid if self.defer_prefill else self._decode
                 dec(q, kv_cache, attn_metadata.block_table[:nd], attn_metadata.seq_lens[:nd], st,
                     max_seq_len=getattr(attn_metadata, "max_seq_len", None), layer=layer, out=o3)
                 return output
+        elif getattr(attn_metadata, "tree_mask", None) is not None:
+            raise NotImplementedError("a tree_mask goes with a decode-only step")
         out = torch.empty(N, self.num_heads, self.head_size, dtype=query.dtype, device=query.device)
         if ndt > 0:
             dec = self._decode_hybrid if self.defer_prefill else self._decode
@@ -471,6 +485,41 @@ class FusedTurboQuantV1Impl(_ImplBase):
                                       scale=self.scale, v_rotate=self.v_rotate, v_lloyd_max=self.v_lloyd_max,
                                       kv_start=ks, num_splits=splits, rotation=st.rotation, out=out, workspace=ws,
                                       sorted_centroids=True, key_fp8=self.key_fp8)
+
+    def _tree(self, q, kv_cache, md, st, layer, out) -> None:
+        """Every request's drafted tokens over their stored slots and, by
+        ``tree_mask``, one another."""
+        if self.defer_prefill:
+            raise NotImplementedError("trees of drafted tokens with TURBOQUANT_DEFER_PREFILL are not supported")
+        N, hq, d = q.shape
+        n = md.max_query_len
+        ks = None
+        if self.sliding_window is not None:
+            pos = getattr(md, "token_positions", None)
+            if pos is None:
+                raise ValueError("a tree_mask on a sliding-window layer needs the metadata's token_positions")
+            if n > self.sliding_window:  # a path could leave the window inside the tree
+                raise NotImplementedError(f"a tree of {n} tokens is larger than the sliding window "
+                                          f"({self.sliding_window})")
+            # [max(0, p - W + 1), context) and the tree's own
+            ks = (pos[:N] - (self.sliding_window - 1)).clamp_(min=0).to(torch.int32)
+        bt, sl, qsl = (t if t.dtype == torch.int32 else t.to(torch.int32)
+                       for t in (md.block_table, md.seq_lens, md.query_start_loc))
+        msl = getattr(md, "max_seq_len", None)
+        msl = msl if msl is not None else bt.shape[1] * kv_cache.shape[1]
+        raw = self._is_raw
+        splits = V1.default_tree_splits(sl.shape[0], n, hq, self.num_kv_heads, d, self.key_bits, self.value_bits, msl)
+        ws = None  # while a graph is captured: from its own pool, so no later step's growth takes it away
+        if not torch.cuda.is_current_stream_capturing():
+            ws = _buf(layer, "ws_tree", (V1.workspace_bytes(N, hq, d, splits),), torch.uint8, q.device)
+        direct = out.is_contiguous() and out.dtype == q.dtype
+        o = V1.v1_tree_attention(q, kv_cache, bt, sl, qsl, None if raw else st.centroids, self.key_bits, self.value_bits,
+                                 tree_mask=md.tree_mask, scale=self.scale, v_rotate=self.v_rotate,
+                                 v_lloyd_max=self.v_lloyd_max, kv_start=ks, num_splits=splits, max_query_len=n,
+                                 max_seq_len=msl, out=out if direct else None, workspace=ws,
+                                 rotation=None if raw else st.rotation, sorted_centroids=True, key_fp8=self.key_fp8)
+        if not direct:
+            out.copy_(o)
 
     def _prefill(self, q, k, v, kv_cache, md, nd, ndt, st):
         """Prefill sequences nd.. of the batch (tokens ndt..N).  A run of

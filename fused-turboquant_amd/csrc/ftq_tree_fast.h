@@ -242,14 +242,19 @@ __global__ __launch_bounds__(256, D <= 128 && CT == 1 ? 3 : 2) void tree_fast_ke
   __shared__ u32x4 pool[2 * B::SIZE > QU ? 2 * B::SIZE : QU];  // two buffers; before: query rows
   __shared__ uint32_t table[F::ENTRIES];
   __shared__ int red[4][2];
+  __shared__ uint32_t sigmas[4];
 
   const int G = a.hq / a.hkv, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const TreeMine mine(a, lane);
-  if constexpr (!F::RAW) {  // pairs of scaled table values
-    const float sg = table_scale<1 << KB>(a.cent, true).sigma;
-    if (tid < F::ENTRIES)
-      table[tid] = f32_to_f16_bits(sg * a.cent[tid & ((1 << KB) - 1)]) | f32_to_f16_bits(sg * a.cent[tid >> KB]) << 16;
+  TreeSigma<F::RAW ? 2 : 1 << KB> scale;
+  float pair[2];
+  if constexpr (!F::RAW) {
+    scale.fetch(a.cent, lane);
+    pair[0] = a.cent[tid & ((1 << KB) - 1)];
+    pair[1] = a.cent[(tid >> KB) & ((1 << KB) - 1)];
+    const uint32_t best = scale.best(lane, wave);
+    if (lane == 0) sigmas[wave] = best;
   }
   TreeUnit u;
   TreePart part;
@@ -264,6 +269,10 @@ __global__ __launch_bounds__(256, D <= 128 && CT == 1 ? 3 : 2) void tree_fast_ke
     W w;
     int first, last;
     w.columns(a, u, part.blk, lane, wave, red, u.len, first, last);  // its barrier: the pool is free
+    if constexpr (!F::RAW) {  // pairs of scaled table values (again for a further block)
+      const float sg = scale.sigma(min(min(sigmas[0], sigmas[1]), min(sigmas[2], sigmas[3])));
+      if (tid < F::ENTRIES) table[tid] = f32_to_f16_bits(sg * pair[0]) | f32_to_f16_bits(sg * pair[1]) << 16;
+    }
     first = min(first, u.ctx) / TK;  // the tree's own positions always
     const int held = (int)min((int64_t)u.len, (int64_t)a.max_blocks << a.lbs);  // positions that can have a page
     const int tb0 = part.part == 0 ? first : max(part.tb0, first), tb1 = min(part.tb1, (held + TK - 1) / TK);

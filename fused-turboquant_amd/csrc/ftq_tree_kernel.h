@@ -111,6 +111,32 @@ struct TreePart {
   int part, spare;          // which of the sequence's; spare: those behind it that do not exist, if it is the last (else 0)
 };
 
+// Over the 64 lanes of a wave, without LDS (the exchanges of wave_min_u32)
+template <typename T>
+__device__ __forceinline__ T tree_wave_sum(T x) {
+  auto dpp = [](T v, auto ctrl) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  x += dpp(x, std::integral_constant<int, 0xB1>{});
+  x += dpp(x, std::integral_constant<int, 0x4E>{});
+  x += dpp(x, std::integral_constant<int, 0x141>{});
+  x += dpp(x, std::integral_constant<int, 0x128>{});
+  auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  x = __builtin_bit_cast(T, (uint32_t)r[0]) + __builtin_bit_cast(T, (uint32_t)r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return __builtin_bit_cast(T, (uint32_t)r[0]) + __builtin_bit_cast(T, (uint32_t)r[1]);
+}
+// Sums of the lanes up to each
+__device__ __forceinline__ int tree_wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);  // lane - 1, - 2, - 4, - 8 of a row of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // rows 1, 3: the row before's last lane
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // rows 2, 3: lane 31
+  return x;
+}
+
 // The parts: no longer than a length for which all sequences together have no more
 // parts than there are workgroups (per head and column block; at least one per
 // sequence), found by bisection to 1/16, a lane per sequence.  The tiles of a sequence
@@ -149,9 +175,7 @@ __device__ __forceinline__ bool tree_share(const TreeArgs& a, const TreeMine& m,
   auto total = [&](auto f) __attribute__((always_inline)) {  // f(tiles) over the sequences
     auto x = f(mine);
     for (int b0 = 64; b0 < a.B; b0 += 64) x += f(tiles(b0 + lane));
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m);
-    return x;
+    return tree_wave_sum(x);
   };
   const int workers = (int)gridDim.x / (a.hkv * a.nblk);  // >= B
   auto parts = [&](int len) __attribute__((always_inline)) {
@@ -159,9 +183,7 @@ __device__ __forceinline__ bool tree_share(const TreeArgs& a, const TreeMine& m,
   };
   int longest = mine;
   for (int b0 = 64; b0 < a.B; b0 += 64) longest = max(longest, tiles(b0 + lane));
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) longest = max(longest, __shfl_xor(longest, m));
-  longest = __builtin_amdgcn_readfirstlane(longest);
+  longest = __builtin_amdgcn_readfirstlane((int)~wave_min_u32(~(uint32_t)longest));
   const float sum = total([](int t) { return (float)t; });
   int lo = max(TREE_PART_MIN, max((longest + a.splits - 1) / a.splits, (int)(sum / (float)workers)));
   lo = __builtin_amdgcn_readfirstlane(lo);
@@ -182,12 +204,7 @@ __device__ __forceinline__ bool tree_share(const TreeArgs& a, const TreeMine& m,
   }
   for (int b0 = 0, before = 0; b0 < a.B; b0 += 64) {
     const int own = (int)((uint32_t)((b0 == 0 ? mine : tiles(b0 + lane)) + hi - 1) / (uint32_t)hi);
-    int c = own;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int o = __shfl_up(c, m);
-      if (lane >= m) c += o;
-    }
+    const int c = tree_wave_scan(own);
     const uint64_t past = __builtin_amdgcn_ballot_w64(before + c > w);
     if (past != 0) {
       const int l = __builtin_ctzll(past), n = __builtin_amdgcn_readlane(own, l);
@@ -287,6 +304,70 @@ __device__ __forceinline__ uint32_t tree_held(const TreeArgs& a, const TreeUnit&
   return on;
 }
 
+// The unnormalised Walsh-Hadamard transform of 4 E values in four lanes
+template <int E>
+__device__ __forceinline__ void tree_fwht(float (&x)[E], int l4) {
+#pragma unroll
+  for (int h = 1; h < E; h <<= 1)
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if ((i & h) == 0) {
+        const float a = x[i], b = x[i + h];
+        x[i] = a + b;
+        x[i + h] = a - b;
+      }
+  const float s1 = l4 & 1 ? -1.f : 1.f, s2 = l4 & 2 ? -1.f : 1.f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) x[i] = __builtin_fmaf(x[i], s1, lane_xor<1>(x[i]));
+#pragma unroll
+  for (int i = 0; i < E; ++i) x[i] = __builtin_fmaf(x[i], s2, lane_xor<2>(x[i]));
+}
+
+// The scale of a table of N values that table_scale finds, the 128 candidates dealt
+// to the four waves (two lanes a candidate, half the table each).
+template <int N>
+struct TreeSigma {
+  float c[N / 2], base;
+  bool none;
+  __device__ __forceinline__ void fetch(const float* cent, int lane) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) c[i] = cent[(lane >> 5) * (N / 2) + i];
+  }
+  __device__ __forceinline__ static void both(float x, float& lo, float& hi) {  // of lanes l and l ^ 32
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    lo = __uint_as_float(r[0]);
+    hi = __uint_as_float(r[1]);
+  }
+  // the wave's best: spread and number
+  __device__ __forceinline__ uint32_t best(int lane, int wave) {
+    float mx = 0.f, x, y;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) mx = fmaxf(mx, fabsf(c[i]));
+    both(mx, x, y);
+    mx = fmaxf(x, y);
+    none = !(mx > 0.f) || !(mx < INFINITY);
+    const int e = (int)((__float_as_uint(mx) >> 23) & 255u);  // mx in [2^(e-127), 2^(e-126))
+    base = __uint_as_float((uint32_t)min(max(263 - e, 1), 254) << 23);  // 2^(136 - e)
+    const int j = wave * 32 + (lane & 31);
+    const float sg = base * (1.f + (float)j * (1.f / 128.f));
+    float tlo = INFINITY, thi = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float t = f16_bits_to_f32(f32_to_f16_bits(sg * c[i])) * __builtin_amdgcn_rcpf(c[i]);
+      tlo = c[i] != 0.f ? fminf(tlo, t) : tlo;
+      thi = c[i] != 0.f ? fmaxf(thi, t) : thi;
+    }
+    both(tlo, x, y);
+    tlo = fminf(x, y);
+    both(thi, x, y);
+    thi = fmaxf(x, y);
+    return wave_min_u32((__float_as_uint((thi - tlo) * __builtin_amdgcn_rcpf(sg)) & ~127u) | (uint32_t)j);
+  }
+  __device__ __forceinline__ float sigma(uint32_t of_all) const {
+    return none ? 1.f : base * (1.f + (float)(of_all & 127u) * (1.f / 128.f));
+  }
+};
+
 // One wave's columns.  KHL: K as f16 hi + lo; NH: f16 parts of the query and of
 // the weights; VHL: V as hi + lo (Lloyd-Max V).
 template <int D, int CT, bool KHL, int NH, bool VHL>
@@ -378,7 +459,6 @@ struct TreeWave {
       float inv = 1.f;
       if (ct < nct) {
         float y[E];
-        const bool on = c0 + 16 * ct + mine < u.n * (a.hq / a.hkv);
         if (a.qt == F32) {
 #pragma unroll
           for (int i = 0; i < E; ++i) y[i] = __uint_as_float(q.x[ct][i >> 2][i & 3]);
@@ -389,26 +469,21 @@ struct TreeWave {
             y[i] = half_bits_to_f32(a.qt == F16 ? F16 : BF16, i & 1 ? w >> 16 : w & 0xffffu);
           }
         }
-#pragma unroll
-        for (int i = 0; i < E; ++i) y[i] = on ? y[i] : 0.f;
         if (a.kb != TREE_RAW) {
           if (a.rot != nullptr) rot_matrix_lanes<D, E>(y, a.rot, rows[mine], l4);
-          else fwht_lanes<E, 4>(y, l4);
+          else tree_fwht(y, l4);
         }
         float mx = 0.f;
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          y[i] *= a.qscale;
-          mx = fmaxf(mx, fabsf(y[i]));
-        }
+        for (int i = 0; i < E; i += 2) asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(mx) : "v"(y[i]), "v"(y[i + 1]));
         mx = fmaxf(mx, lane_xor<1>(mx));
-        mx = fmaxf(mx, lane_xor<2>(mx));
+        mx = fmaxf(mx, lane_xor<2>(mx)) * fabsf(a.qscale);
         // A query that f16 cannot hold is scaled to [2^13, 2^14).  Small ones need
         // no scale: what their low parts lose below f16's range is 2^-25 of a
         // score, an absolute error.
         const int e = (int)((__float_as_uint(mx) >> 23) & 255u);
         const int ue = e >= 127 + 14 && e < 255 ? 140 + 127 - e : 127;
-        const float up = __uint_as_float((uint32_t)ue << 23);
+        const float up = a.qscale * __uint_as_float((uint32_t)ue << 23);
         inv = __shfl(__uint_as_float((uint32_t)(254 - ue) << 23), n << 2);  // column n's
 #pragma unroll
         for (int i = 0; i < E; ++i) rows[mine][l4 * E + i] = y[i] * up;

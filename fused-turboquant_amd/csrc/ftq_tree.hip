@@ -270,14 +270,20 @@ hipError_t tree_launch(const TreeArgs& a, int ct, unsigned grid, int64_t tokens,
 }
 
 // 16-column tiles of a wave for sequences of at most `cols` columns: one where 64
-// columns do (fewer registers, more workgroups a CU).
+// columns do (24 sequences, 20 columns of 64-wide heads: 47 us with three workgroups
+// a CU, 53 before), else two (16 sequences of 1024-6000 positions, 128 columns of
+// 128-wide heads: 91 us, with one 102; 98000 positions, 244 columns: 339 and 448).
 int tree_ct(int d, int64_t cols) { return d == 256 || cols <= 64 ? 1 : 2; }
-// Parts (TreeShare) of all sequences together, per kv head and column block: what the
-// 256 CUs hold at once (three workgroups a CU with one column tile a wave below
-// d = 256, else two); where that is hardly more than the sequences, three rounds of it or more.
+// Workgroups that the 256 CUs hold at once, by registers and LDS.
+int64_t tree_resident(int d, int ct) { return 256 * (d != 256 && ct == 1 ? 3 : 2); }
+// Parts (tree_share) of all sequences together, per kv head and column block: what the
+// GPU holds.  (Half of it: 91 -> 124 us at 16 sequences of 1024-6000 positions; twice:
+// 111 us, each part's start and end are work too.)  Where that is hardly more than the
+// sequences, two each (48 sequences of 3000 positions, 128 columns: 201 us, with one
+// each 206, with three 223).
 int64_t tree_parts_all(int d, int ct, int hkv, int64_t nblk, int64_t batch) {
-  const int64_t s = 256 * (d != 256 && ct == 1 ? 3 : 2) / (hkv * nblk);
-  return 3 * batch <= 2 * s ? s : 3 * batch;
+  const int64_t s = tree_resident(d, ct) / (hkv * nblk);
+  return 3 * batch <= 2 * s ? s : std::max(s, 2 * batch);
 }
 
 }  // namespace
@@ -295,7 +301,9 @@ extern "C" int ftq_v1_tree_choose_splits(int batch, int max_query_len, int num_q
   const int64_t ncols = (int64_t)max_query_len * (num_q_heads / num_kv_heads);
   const int ct = tree_ct(d, ncols);
   const int64_t nblk = (ncols + 64 * ct - 1) / (64 * ct);
-  if (nblk * batch * num_kv_heads >= 2048) return 1;  // four rounds of whole sequences
+  // Two rounds of whole sequences need no parts: 200 sequences of 500-4480 positions,
+  // 32 columns: 391 us, in parts 433; 128 sequences (1.3 rounds): 365 and 330.
+  if (nblk * batch * num_kv_heads >= 2 * tree_resident(d, ct)) return 1;
   const int64_t tiles = ((int64_t)max_seq_len + (d == 64 ? 63 : 31)) / (d == 64 ? 64 : 32);
   const int64_t s = 3 * tree_parts_all(d, ct, num_kv_heads, nblk, batch) / batch + 1;
   return (int)std::max<int64_t>(std::min({s, tiles / TREE_PART_MIN, (int64_t)64}), 1);

@@ -41,14 +41,15 @@ __device__ __forceinline__ float pow2_of(float mx) {
 }
 
 // Any slot format: the tile's slots as rows of LDS, from them the factors of each
-// position, then the operands.  Every product is float32-level (hi + lo parts of
-// what f16 does not hold exactly).  Bound by the LDS reads and bit extractions of
+// position, then the operands.  FULL: every product is float32-level (hi + lo parts
+// of what f16 does not hold exactly); else, for bf16 outputs, one part: a rounding of
+// 2^-12 at each operand beside the output's 2^-9.  Bound by the LDS reads and bit extractions of
 // its dequantisation; the formats in everyday use have kernels of their own.
-template <int D, bool LM>
-__global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
+template <int D, bool LM, bool FULL>
+__global__ __launch_bounds__(256, FULL ? 1 : 2) void tree_any_kernel(const TreeArgs a) {
   using C = TreeGeo<D>;
   constexpr int CT = C::CT, TK = C::TK, NS = C::NS, NB = C::NB, NT = C::NT, NP = C::NP;
-  using W = TreeWave<D, CT, true, 2, LM>;
+  using W = TreeWave<D, CT, FULL, FULL ? 2 : 1, LM && FULL>;
   constexpr int LPT = 256 / TK, DPL = D / LPT;  // lanes of a position, their dims
   extern __shared__ __attribute__((aligned(16))) uint32_t pool[];  // slots [TK][pitch]; before: query rows; both: operands behind
   __shared__ __attribute__((aligned(16))) float tb[2][TK];
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
       __syncthreads();
       for (int i = tid; i < NT * NS * 64; i += 256) {
         const int l = i & 63, ts = i >> 6, m = l & 15, g = l >> 4;
-        const int d0 = (ts % NS) * 32 + 8 * g, at = (ts / NS) * 2 * NS * 64 + C::kunit(ts % NS, m, g);
+        const int d0 = (ts % NS) * 32 + 8 * g, at = (ts / NS) * W::KP * NS * 64 + C::kunit(ts % NS, m, g);
         const uint32_t* row = rows + ((ts / NS) * 16 + m) * pitch;
         uint32_t h[4], lo[4];
 #pragma unroll
@@ -184,7 +185,7 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
           }
         }
         kf[at] = u32x4{h[0], h[1], h[2], h[3]};
-        kf[at + NS * 64] = u32x4{lo[0], lo[1], lo[2], lo[3]};
+        if constexpr (FULL) kf[at + NS * 64] = u32x4{lo[0], lo[1], lo[2], lo[3]};
       }
       for (int i = tid; i < NP * NB * 64; i += 256) {
         const int l = i & 63, pb = i >> 6, m = l & 15, g = l >> 4, d = NB * m + pb % NB;
@@ -202,17 +203,17 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
             } else if constexpr (LM) {
               const uint32_t c = tabv[row_bits(row, 8 * geo.kps + d * 4, 4)];
               x[k] = f16_bits_to_f32(c & 0xffffu) * vex[p];
-              y[k] = f16_bits_to_f32(c >> 16) * vex[p];
+              if constexpr (FULL) y[k] = f16_bits_to_f32(c >> 16) * vex[p];
             } else {
               x[k] = ((float)row_bits(row, 8 * geo.kps + d * a.vb, a.vb) - mid) * vex[p];
             }
           }
           h[j] = pk_f16(x[0], x[1]);
-          if constexpr (LM) lo[j] = pk_f16(y[0], y[1]);
+          if constexpr (LM && FULL) lo[j] = pk_f16(y[0], y[1]);
         }
         const int at = ((pb / NB) * W::VP * NB + pb % NB) * 64 + l;
         vf[at] = u32x4{h[0], h[1], h[2], h[3]};
-        if constexpr (LM) vf[at + NB * 64] = u32x4{lo[0], lo[1], lo[2], lo[3]};
+        if constexpr (LM && FULL) vf[at + NB * 64] = u32x4{lo[0], lo[1], lo[2], lo[3]};
       }
       __syncthreads();
       const uint32_t on = tree_held<TK>(a, u, pos0);  // bit k: positions 16 k .. of the tile have a page
@@ -223,16 +224,16 @@ __global__ __launch_bounds__(256, 1) void tree_any_kernel(const TreeArgs a) {
   }
 }
 
-template <int D, bool LM>
+template <int D, bool LM, bool FULL>
 hipError_t any_launch(const TreeArgs& a, unsigned grid, hipStream_t st) {
   using C = TreeGeo<D>;
-  using W = TreeWave<D, C::CT, true, 2, LM>;
+  using W = TreeWave<D, C::CT, FULL, FULL ? 2 : 1, LM && FULL>;
   const bool raw = a.kb == TREE_RAW;
   const V1Geom geo = raw ? V1Geom{2 * D, 2 * D, 2 * D, 4 * D} : v1_geom(D, a.kb, a.vb, (a.flags & V1F_KFP8) != 0);
   const int pitch = ((geo.raw + 3) / 4 + 1) | 1;
   const size_t rows = (size_t)(C::TK * pitch + 3) / 4 * 16;
   const size_t lds = std::max(rows + (size_t)(W::KU + W::VU) * 16, (size_t)64 * (D + 4) * 4);
-  tree_any_kernel<D, LM><<<dim3(grid), dim3(256), lds, st>>>(a);
+  tree_any_kernel<D, LM, FULL><<<dim3(grid), dim3(256), lds, st>>>(a);
   return hipGetLastError();
 }
 
@@ -264,7 +265,8 @@ template <int D>
 hipError_t tree_launch(const TreeArgs& a, int ct, unsigned grid, int64_t tokens, bool vrot, hipStream_t st) {
   const bool lm = (a.flags & V1F_VLM) != 0 && a.vb == 4;
   const hipError_t e = tree_fast_takes(a) ? (D == 64 ? tree_fast_64(a, ct, grid, st) : D == 128 ? tree_fast_128(a, ct, grid, st) : tree_fast_256(a, ct, grid, st))
-                       : lm ? any_launch<D, true>(a, grid, st) : any_launch<D, false>(a, grid, st);
+                       : a.ot == BF16 ? (lm ? any_launch<D, true, false>(a, grid, st) : any_launch<D, false, false>(a, grid, st))
+                       : lm ? any_launch<D, true, true>(a, grid, st) : any_launch<D, false, true>(a, grid, st);
   if (e != hipSuccess || a.wo == nullptr) return e;
   return tree_merge<D>(a, tokens, vrot, st);
 }

@@ -3,8 +3,10 @@
 // and slots (from the requests' lengths, with a free list on the device), the
 // accepted path of each drafted tree, and the move of the accepted slots to
 // consecutive positions.  Whole numbers and bytes only; all three are bound by
-// latency (a few dependent reads) at a decode step's sizes, and the maps by
-// their writes at a prompt's.
+// latency (a few dependent reads) at a decode step's sizes.  Kernel times on one
+// MI355X: tables of 64 requests with a tree of 8 nodes, pages taken and given back,
+// 8.4 us; of nine prompts with up to 4096 tokens 5.1 and 5.5 us (pages, then tokens);
+// a call from Python takes 12-19 us of host time, which covers them.
 #include "ftq_device.h"
 #include "ftq_internal.h"
 
@@ -178,7 +180,9 @@ __global__ __launch_bounds__(1024) void step_alloc_kernel(const StepArgs a, int 
 }
 
 // One wave per tree: its nodes in LDS, then from the root the lowest child whose
-// token is the answer at the current node.
+// token is the answer at the current node, 64 nodes at a time.  Latency of the loads
+// and of a step per accepted node: 2.3 us for three trees of 8 nodes, 4.7 for 64
+// of 61.
 __global__ __launch_bounds__(64) void tree_accept_kernel(const int64_t* __restrict__ tokens, const int32_t* __restrict__ parents,
                                                          const int64_t* __restrict__ targets, const int32_t* __restrict__ qsl,
                                                          int64_t num_tokens, int width, int32_t* __restrict__ path,
@@ -240,7 +244,8 @@ struct CommitArgs {
 // of a sequence's slots in one layer.  The path ascends, so path[j] >= j and no
 // piece is overwritten before it is read: a thread moves the same piece of every
 // position, and reads a group of four before it writes them (what it writes lies
-// at or below what it reads).
+// at or below what it reads).  All layers in one launch: 3.1 MB moved in 32 layers in
+// 7.3 us, most of it the latency of path, table and slot in turn.
 template <typename T>
 __global__ __launch_bounds__(256) void commit_slots_kernel(const CommitArgs a) {
   constexpr int NP = 256;  // path entries at a time

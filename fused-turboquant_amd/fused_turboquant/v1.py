@@ -515,7 +515,8 @@ def v1_tree_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: 
     ``key_bits = value_bits = RAW_BITS`` reads raw fp16 slots (``centroids``
     None); every other format of ``v1_decode_attention`` is taken.
     ``max_query_len`` and ``max_seq_len`` (host numbers, default T and the
-    table's width) only size the launch and ``num_splits``; ``workspace``
+    table's width) only size the launch and ``num_splits``, the most parts a
+    sequence's positions are cut into (1: no second launch); ``workspace``
     (uint8, ``workspace_bytes(T, ...)``) may be preallocated for graph capture.
     ``lse`` (float32 [T, Hq]) as in ``v1_decode_attention``.
     """

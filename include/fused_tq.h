@@ -422,6 +422,8 @@ int ftq_v1_chunk_attention(const void* query, int q_dtype, const uint8_t* kv_cac
  *   key_bits, value_bits, v_flags: as ftq_v1_decode_attention (bits 0, 1 and
  *   2), or both 16 for raw fp16 slots (no flags, no rotation, no centroids)
  *   max_query_len: the longest sequence's tokens; sizes the grid only
+ *   num_splits: 1, or the most parts that a sequence's positions are cut into
+ *   (the parts are made of one length for all sequences, on the device)
  *   workspace: ftq_v1_workspace_bytes(num_tokens, num_q_heads, d, num_splits)
  * One launch with one split (unless a caller's matrix un-rotates the output),
  * else two.  No counterpart in the reference, which decodes one token a

@@ -47,8 +47,9 @@ __device__ __forceinline__ void step_token(const StepArgs& a, const int* qsl, in
   int b = -1;
   if (t >= qsl[0] && t < qsl[a.B]) {
     b = find_below(qsl, 0, a.B, (int)t);
-    const int i = (int)t - qsl[b], past = max(a.past[b], 0), at = past + i;
-    const int page = at / a.bs, limit = a.have != nullptr ? a.have[b] : a.max_blocks;
+    const int i = (int)t - qsl[b], past = max(a.past[b], 0);
+    const int64_t at = (int64_t)past + i, page = at / a.bs;
+    const int limit = a.have != nullptr ? a.have[b] : a.max_blocks;
     const int id = page < limit ? a.bt[b * a.bt_row + page] : -1;
     if (id >= 0) slot = (int64_t)id * a.bs + (at - page * a.bs);
     pos = past + (int64_t)(a.depths != nullptr ? a.depths[t] : i);
@@ -58,7 +59,11 @@ __device__ __forceinline__ void step_token(const StepArgs& a, const int* qsl, in
   a.req[t] = b;
 }
 
-__device__ __forceinline__ int step_len(const StepArgs& a, int i) { return max(a.past[i], 0) + max(a.qsl[i + 1] - a.qsl[i], 0); }
+// of a request; past 2^31 - 1: that
+__device__ __forceinline__ int step_len(const StepArgs& a, int i) {
+  const int64_t n = (int64_t)a.qsl[i + 1] - a.qsl[i], len = (int64_t)max(a.past[i], 0) + (n > 0 ? n : 0);
+  return (int)(len < 0x7fffffff ? len : 0x7fffffff);
+}
 
 // Without a free list: a workgroup per 1024 tokens.
 __global__ __launch_bounds__(256) void step_map_kernel(const StepArgs a) {
@@ -308,6 +313,7 @@ extern "C" int ftq_step_tables(const int32_t* query_start_loc, const int32_t* pa
   const bool alloc = num_blocks_held != nullptr || free_blocks != nullptr || free_count != nullptr;
   FTQ_REQUIRE(!alloc || ((num_blocks_held || batch == 0) && free_count && (free_blocks || pool_size == 0)),
               "step tables: num_blocks, free_blocks and free_count go together");
+  FTQ_REQUIRE(!alloc || (int64_t)batch * max_blocks <= INT32_MAX - pool_size, "step tables: too many table entries");
   FTQ_REQUIRE(missing && query_start_loc, "null pointer argument");
   FTQ_REQUIRE(batch == 0 || (past_lens && seq_lens && (block_table || max_blocks == 0)), "null pointer argument");
   FTQ_REQUIRE(num_tokens == 0 || (slot_mapping && positions && token_request), "null pointer argument");

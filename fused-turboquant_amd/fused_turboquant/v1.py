@@ -553,7 +553,8 @@ def v1_tree_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: 
         raise ValueError("lse must be a contiguous float32 tensor of T * num_q_heads entries")
     if max_query_len is not None and (max_query_len < 0 or (max_query_len == 0 and T > 0)):
         raise ValueError("max_query_len must be positive")
-    dev = _lib.require_device(query, kv_cache, block_table, seq_lens, query_start_loc, centroids, tree_mask, kv_start, lse)
+    dev = _lib.require_device(query, kv_cache, block_table, seq_lens, query_start_loc, centroids, tree_mask, kv_start, lse, out,
+                              workspace)
     q = query.contiguous()
     if q.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         q = q.float()

@@ -471,7 +471,8 @@ class ModelRunner:
 
     def tree_step(self, drafted: torch.Tensor):
         """One step: ``drafted`` (int64 [B, n - 1]) are the tokens of the nodes
-        behind the root.  Each request gains one token or more, until it has
+        behind the root, below the vocabulary's size; -1 for a node with none,
+        which is never accepted.  Each request gains one token or more, until it has
         its ``max_tokens``."""
         st = self._st
         if tuple(drafted.shape) != (st.nodes.shape[0], st.nodes.shape[1] - 1):

@@ -275,8 +275,9 @@ hipError_t tree_launch(const TreeArgs& a, int ct, unsigned grid, int64_t tokens,
 }
 
 // 16-column tiles of a wave for sequences of at most `cols` columns: one where 64
-// columns do (24 sequences, 20 columns of 64-wide heads: 47 us with three workgroups
-// a CU, 53 before), else two (16 sequences of 1024-6000 positions, 128 columns of
+// columns do, and three workgroups a CU (24 sequences, 20 columns of 64-wide heads: 54
+// us, with two column tiles 62, with one and two workgroups 61; 80 sequences, 32
+// columns of 128-wide heads: 235, 279 and 276), else two (16 sequences of 1024-6000 positions, 128 columns of
 // 128-wide heads: 91 us, with one 102; 98000 positions, 244 columns: 339 and 448).
 int tree_ct(int d, int64_t cols) { return d == 256 || cols <= 64 ? 1 : 2; }
 // Workgroups that the 256 CUs hold at once, by registers and LDS.

@@ -17,7 +17,7 @@
 // vector and matrix instructions interleaved by hand (98000 positions: 340 -> 362 us),
 // wave priorities around the products (340 -> 344).
 // Operands: K table values as f16 (a common scale that keeps their relative
-// errors alike, table_scale), V codes exact (centred, times the scale's own power
+// errors alike, TreeSigma), V codes exact (centred, times the scale's own power
 // of two).  bf16 outputs: query and weights as one f16 number, 2^-11 beside the
 // output's 2^-8; fp16 outputs: as hi + lo.
 #pragma once

@@ -42,11 +42,11 @@ __device__ __forceinline__ float pow2_of(float mx) {
 
 // Any slot format: the tile's slots as rows of LDS, from them the factors of each
 // position, then the operands.  FULL: every product is float32-level (hi + lo parts
-// of what f16 does not hold exactly); else, for bf16 outputs, one part (rounded by at
-// most 2^-11 of a K table value, query or weight, beside 2^-8 of the output) and
-// two workgroups a CU.  Bound by the LDS reads and bit extractions of its
+// of what f16 does not hold exactly); else, for bf16 outputs of 16-bit queries, one
+// part (rounded by at most 2^-11 of a K table value, query or weight, beside 2^-8 of
+// the output) and two workgroups a CU.  Bound by the LDS reads and bit extractions of its
 // dequantisation: 16 sequences of 1024-5989 positions, 32 nodes, 128-wide heads, 8-bit
-// codes: 313 us for bf16 (FULL: 530), where 4-bit ones take 91 in a kernel of the
+// codes: 333 us for bf16 (FULL: 530), where 4-bit ones take 88 in a kernel of the
 // formats in everyday use.
 template <int D, bool LM, bool FULL>
 __global__ __launch_bounds__(256, FULL ? 1 : 2) void tree_any_kernel(const TreeArgs a) {
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256, FULL ? 1 : 2) void tree_any_kernel(const TreeA
     w.columns(a, u, part.blk, lane, wave, red, u.len, first, last);  // its barrier: the pool is free, and the tables written
     typename W::Raw q;
     w.fetch(a, u, lane, q);
-    w.queries(a, u, q, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
+    w.template queries<-1>(a, u, q, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
     __syncthreads();
     first = min(first, u.ctx) / TK;  // the tree's own positions always
     const int tb0 = part.part == 0 ? first : max(part.tb0, first), tb1 = part.tb1;
@@ -256,10 +256,10 @@ hipError_t tree_merge(const TreeArgs& a, int64_t tokens, bool vrot, hipStream_t 
 #undef FTQ_TREE_MERGE
 }
 
-// The formats of ftq_tree_fast.h: 16-bit outputs, 2-4 bit codes or raw slots that
+// The formats of ftq_tree_fast.h: 16-bit queries and outputs, 2-4 bit codes or raw slots that
 // 16-byte loads reach, and positions of a tile within 32-bit offsets.
 bool tree_fast_takes(const TreeArgs& a) {
-  if (a.ot == F32 || a.spos > (1 << 26)) return false;
+  if (a.ot == F32 || a.qt == F32 || a.spos > (1 << 26)) return false;
   if (a.kb == TREE_RAW) return (((uintptr_t)a.cache | (uintptr_t)a.sblk | (uintptr_t)a.spos | (uintptr_t)a.shead) & 15) == 0;
   return a.kb >= 2 && a.kb <= 4 && a.vb >= 2 && a.vb <= 4 && (a.flags & V1F_KFP8) == 0 && !((a.flags & V1F_VLM) != 0 && a.vb == 4);
 }
@@ -268,7 +268,7 @@ template <int D>
 hipError_t tree_launch(const TreeArgs& a, int ct, unsigned grid, int64_t tokens, bool vrot, hipStream_t st) {
   const bool lm = (a.flags & V1F_VLM) != 0 && a.vb == 4;
   const hipError_t e = tree_fast_takes(a) ? (D == 64 ? tree_fast_64(a, ct, grid, st) : D == 128 ? tree_fast_128(a, ct, grid, st) : tree_fast_256(a, ct, grid, st))
-                       : a.ot == BF16 ? (lm ? any_launch<D, true, false>(a, grid, st) : any_launch<D, false, false>(a, grid, st))
+                       : a.ot == BF16 && a.qt != F32 ? (lm ? any_launch<D, true, false>(a, grid, st) : any_launch<D, false, false>(a, grid, st))
                        : lm ? any_launch<D, true, true>(a, grid, st) : any_launch<D, false, true>(a, grid, st);
   if (e != hipSuccess || a.wo == nullptr) return e;
   return tree_merge<D>(a, tokens, vrot, st);
@@ -360,7 +360,7 @@ extern "C" int ftq_v1_tree_attention(const void* query, int q_dtype, int64_t num
   FTQ_REQUIRE(need >= 0 && workspace_bytes >= need, "workspace too small (see ftq_v1_workspace_bytes)");
   const int64_t ncols = std::min<int64_t>(max_query_len, num_tokens) * (num_q_heads / num_kv_heads);
   TreeArgs a{};
-  a.ot = out_dtype; a.kb = key_bits; a.vb = value_bits; a.flags = v_flags;
+  a.qt = q_dtype; a.ot = out_dtype; a.kb = key_bits; a.vb = value_bits; a.flags = v_flags;
   a.cache = kv_cache; a.nb = num_blocks; a.sblk = stride_block; a.spos = stride_pos; a.shead = stride_head;
   const int ct = tree_fast_takes(a) ? tree_ct(d, ncols) : tree_ct(d, INT32_MAX);
   const int64_t nblk = (ncols + 64 * ct - 1) / (64 * ct);
@@ -368,7 +368,7 @@ extern "C" int ftq_v1_tree_attention(const void* query, int q_dtype, int64_t num
   int64_t grid = 0;
   FTQ_REQUIRE(!__builtin_mul_overflow(nblk * num_kv_heads, parts, &grid) && grid <= INT32_MAX, "tree attention: grid too large");
   const bool vrot = (v_flags & V1F_VROT) != 0;
-  a.q = query; a.qt = q_dtype; a.tokens = (int)num_tokens;
+  a.q = query; a.tokens = (int)num_tokens;
   while ((1 << a.lbs) < block_size) ++a.lbs;
   a.bt = block_table; a.max_blocks = max_blocks_per_seq;
   a.sl = seq_lens; a.qsl = query_start_loc; a.ks = kv_start;

@@ -1,6 +1,6 @@
 // Tree attention for the formats in everyday use: 2-4 bit keys (codebook) with
-// 2-4 bit uniform values, and raw fp16 slots, with 16-bit outputs (float32
-// outputs take the kernel of ftq_tree.hip, whose products are all float32-level).
+// 2-4 bit uniform values, and raw fp16 slots, with 16-bit queries and outputs
+// (float32 ones take the kernel of ftq_tree.hip, whose products are all float32-level).
 //
 // Two LDS buffers of operands: while the waves multiply one tile, each thread
 // turns the bytes of the next, which it loaded a tile earlier, into operands, and
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(256, D <= 128 && CT == 1 ? 3 : 2) void tree_fast_ke
     if (tb0 < tb1) entries(tb0);
     w.fetch(a, u, lane, q);
     if (tb0 < tb1) fetch(tb0);
-    w.queries(a, u, q, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
+    w.template queries<F::RAW ? 1 : 0>(a, u, q, lane, reinterpret_cast<float(*)[D + 4]>(pool) + 16 * wave);
     __syncthreads();
     if (tid < 2 * 64 * NP) pool[tid / (64 * NP) * B::SIZE + B::X + tid % (64 * NP)] = u32x4{0, 0, 0, 0};
     __syncthreads();

@@ -76,6 +76,7 @@ struct TreeArgs {
   const float* rot;         // matrix of the rotation strategy, or null
 };
 
+typedef __bf16 TreeBf8 __attribute__((ext_vector_type(8)));
 constexpr int TREE_RAW = 16;  // key_bits of raw fp16 slots
 
 template <int D> struct TreeGeo {
@@ -314,25 +315,6 @@ __device__ __forceinline__ uint32_t tree_held(const TreeArgs& a, const TreeUnit&
   return on;
 }
 
-// The unnormalised Walsh-Hadamard transform of 4 E values in four lanes
-template <int E>
-__device__ __forceinline__ void tree_fwht(float (&x)[E], int l4) {
-#pragma unroll
-  for (int h = 1; h < E; h <<= 1)
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-      if ((i & h) == 0) {
-        const float a = x[i], b = x[i + h];
-        x[i] = a + b;
-        x[i + h] = a - b;
-      }
-  const float s1 = l4 & 1 ? -1.f : 1.f, s2 = l4 & 2 ? -1.f : 1.f;
-#pragma unroll
-  for (int i = 0; i < E; ++i) x[i] = __builtin_fmaf(x[i], s1, lane_xor<1>(x[i]));
-#pragma unroll
-  for (int i = 0; i < E; ++i) x[i] = __builtin_fmaf(x[i], s2, lane_xor<2>(x[i]));
-}
-
 // The scale of a table of N values that table_scale finds, the 128 candidates dealt
 // to the four waves (two lanes a candidate, half the table each).
 template <int N>
@@ -378,7 +360,7 @@ struct TreeSigma {
   }
 };
 
-// One wave's columns.  KHL: K as f16 hi + lo; NH: f16 parts of the query and of
+// One wave's columns.  KHL: K as f16 hi + lo, and float32 queries too (else 16-bit ones); NH: f16 parts of the query and of
 // the weights; VHL: V as hi + lo (Lloyd-Max V).
 template <int D, int CT, bool KHL, int NH, bool VHL>
 struct TreeWave {
@@ -436,82 +418,160 @@ struct TreeWave {
     last = __builtin_amdgcn_readfirstlane(max(max(red[0][1], red[1][1]), max(red[2][1], red[3][1])));
   }
 
-  // The columns' queries as they are stored; four lanes per query
+  // The columns' queries as they are stored: lane (n, g) dims 32 s + 8 g + j of column n
   struct Raw {
-    static constexpr int E = D / 4;
-    u32x4 x[CT][E / 4];
+    u32x4 x[CT][NS][KHL ? 2 : 1];  // float32: j < 4 and the others; 16 bits: all in the first
   };
   __device__ __forceinline__ void fetch(const TreeArgs& a, const TreeUnit& u, int lane, Raw& q) {
-    constexpr int E = Raw::E;
     const int G = a.hq / a.hkv;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const int col = min(c0 + 16 * ct + (lane >> 2), u.n * G - 1);  // behind the last: it again, for nobody
+      const int col = min(c0 + 16 * ct + (lane & 15), u.n * G - 1);  // behind the last: it again, for nobody
       const int r = col / G, h = u.kvh * G + (col - r * G);
-      const int64_t off = ((int64_t)(u.q0 + r) * a.hq + h) * D + (lane & 3) * E;
-      const u32x4* src = reinterpret_cast<const u32x4*>(static_cast<const char*>(a.q) + off * (a.qt == F32 ? 4 : 2));
+      const int64_t off = ((int64_t)(u.q0 + r) * a.hq + h) * D + 8 * (lane >> 4);
+      const char* src = static_cast<const char*>(a.q) + off * (a.qt == F32 ? 4 : 2);
+      if (KHL && a.qt == F32) {
 #pragma unroll
-      for (int i = 0; i < E / 8; ++i) q.x[ct][i] = src[i];
+        for (int s = 0; s < NS; ++s)
 #pragma unroll
-      for (int i = E / 8; i < E / 4; ++i) q.x[ct][i] = a.qt == F32 ? src[i] : u32x4{0, 0, 0, 0};
+          for (int k = 0; k < KP; ++k) q.x[ct][s][k] = *reinterpret_cast<const u32x4*>(src + 128 * s + 16 * k);
+      } else {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          q.x[ct][s][0] = *reinterpret_cast<const u32x4*>(src + 64 * s);
+          if constexpr (KHL) q.x[ct][s][1] = u32x4{0, 0, 0, 0};
+        }
+      }
     }
   }
 
-  // The columns' queries, rotated and scaled, as f16 hi + lo, through 16 rows of LDS
-  // of the wave's own.  Four lanes per query: most butterflies of the transform stay
-  // inside a lane.
+  // The columns' queries, rotated and scaled, as f16 hi + lo.  The transform is a matrix
+  // product, its rows in the order in which the score products take a query's dims (block
+  // b: dims 32 (b >> 1) + 8 g + 4 (b & 1) + i); a float32 query goes in as three bf16
+  // numbers, which is exact.  A caller's matrix: through 16 rows of LDS of the wave's own.
+  // RAW: 1 raw slots (no transform), 0 codes, -1 either.
+  template <int RAW>
   __device__ __forceinline__ void queries(const TreeArgs& a, const TreeUnit& u, const Raw& q, int lane, float (*rows)[D + 4]) {
-    constexpr int E = D / 4;
-    const int l4 = lane & 3, mine = lane >> 2, g = lane >> 4, n = lane & 15;
+    const int g = lane >> 4, n = lane & 15;
+    // signs of row n and dims 8 g + j (the parity of the bits that both have), ones of
+    // the operand's type
+    const uint32_t one = a.qt == F16 ? 0x3c003c00u : 0x3f803f80u;
+    const int hg = __builtin_popcount((n >> 2) & g), n0 = n & 1, n1 = (n >> 1) & 1;
+    auto pair = [&](int j0, int j1) { return one | (uint32_t)(j0 & 1) << 15 | (uint32_t)(j1 & 1) << 31; };
+    const uint32_t e0 = pair(hg, hg + n0), e1 = pair(hg + n1, hg + n0 + n1), sgn = 0x80008000u;
     qlarge = 0;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       float inv = 1.f;
+      floatx4 y[NB];  // dims 32 (b >> 1) + 8 g + 4 (b & 1) + i of column n
+#pragma unroll
+      for (int b = 0; b < NB; ++b) y[b] = floatx4{0.f, 0.f, 0.f, 0.f};
       if (ct < nct) {
-        float y[E];
-        if (a.qt == F32) {
+        if (RAW == 1 || (RAW < 0 && a.kb == TREE_RAW) || a.rot != nullptr) {
+          if (KHL && a.qt == F32) {
 #pragma unroll
-          for (int i = 0; i < E; ++i) y[i] = __uint_as_float(q.x[ct][i >> 2][i & 3]);
-        } else {
+            for (int b = 0; b < NB; ++b) y[b] = __builtin_bit_cast(floatx4, q.x[ct][b >> 1][KHL ? b & 1 : 0]);
+          } else {
 #pragma unroll
-          for (int i = 0; i < E; ++i) {
-            const uint32_t w = q.x[ct][i >> 3][(i >> 1) & 3];
-            y[i] = half_bits_to_f32(a.qt == F16 ? F16 : BF16, i & 1 ? w >> 16 : w & 0xffffu);
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t w = q.x[ct][b >> 1][0][2 * (b & 1) + (i >> 1)];
+                y[b][i] = half_bits_to_f32(a.qt == F16 ? F16 : BF16, i & 1 ? w >> 16 : w & 0xffffu);
+              }
           }
-        }
-        if (a.kb != TREE_RAW) {
-          if (a.rot != nullptr) rot_matrix_lanes<D, E>(y, a.rot, rows[mine], l4);
-          else tree_fwht(y, l4);
+          if (RAW != 1 && a.rot != nullptr) {
+            const int d0 = 8 * g;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              *reinterpret_cast<floatx4*>(&rows[n][32 * (b >> 1) + d0 + 4 * (b & 1)]) = y[b];
+              y[b] = floatx4{0.f, 0.f, 0.f, 0.f};
+            }
+            __asm__ volatile("" ::: "memory");  // a wave's LDS accesses run in order
+            for (int k = 0; k < D; ++k) {
+              const float xk = rows[n][k];
+#pragma unroll
+              for (int b = 0; b < NB; ++b) {
+                const floatx4 m = *reinterpret_cast<const floatx4*>(a.rot + (int64_t)k * D + 32 * (b >> 1) + d0 + 4 * (b & 1));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[b][i] = __builtin_fmaf(xk, m[i], y[b][i]);
+              }
+            }
+            __asm__ volatile("" ::: "memory");
+          }
+        } else {
+          [[maybe_unused]] auto transform = [&](auto wide, auto part) __attribute__((always_inline)) {  // y += H x
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+              for (int s = 0; s < NS; ++s) {
+                const uint32_t all = __builtin_popcount((b >> 1) & s) & 1 ? sgn : 0u, up = b & 1 ? sgn : 0u;
+                const u32x4 h{e0 ^ all, e1 ^ all, e0 ^ all ^ up, e1 ^ all ^ up};
+                if constexpr (decltype(wide)::value)
+                  y[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(TreeBf8, h), __builtin_bit_cast(TreeBf8, part(s)), y[b], 0, 0, 0);
+                else
+                  y[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, h), __builtin_bit_cast(half8, part(s)), y[b], 0, 0, 0);
+              }
+          };
+          if (a.qt == F16) {
+            transform(std::false_type{}, [&](int s) { return q.x[ct][s][0]; });
+          } else if (!KHL || a.qt == BF16) {
+            transform(std::true_type{}, [&](int s) { return q.x[ct][s][0]; });
+          } else if constexpr (KHL) {
+            u32x4 rest[NS][2];
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) rest[s][k] = q.x[ct][s][k];
+#pragma unroll 1
+            for (int t = 0; t < 3; ++t) {
+              u32x4 top[NS];  // the upper halves, and what they leave
+#pragma unroll
+              for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                  for (int i = 0; i < 4; i += 2) {
+                    const uint32_t v0 = rest[s][k][i], v1 = rest[s][k][i + 1];
+                    top[s][2 * k + i / 2] = __builtin_amdgcn_perm(v1, v0, 0x07060302u);
+                    rest[s][k][i] = __float_as_uint(__uint_as_float(v0) - __uint_as_float(v0 & 0xffff0000u));
+                    rest[s][k][i + 1] = __float_as_uint(__uint_as_float(v1) - __uint_as_float(v1 & 0xffff0000u));
+                  }
+              transform(std::true_type{}, [&](int s) { return top[s]; });
+            }
+          }
         }
         float mx = 0.f;
 #pragma unroll
-        for (int i = 0; i < E; i += 2) asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(mx) : "v"(y[i]), "v"(y[i + 1]));
-        mx = fmaxf(mx, lane_xor<1>(mx));
-        mx = fmaxf(mx, lane_xor<2>(mx)) * fabsf(a.qscale);
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const float v0 = y[b][i], v1 = y[b][i + 1];
+            asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(mx) : "v"(v0), "v"(v1));
+          }
+        mx = warp_max_q(mx) * fabsf(a.qscale);
         // A query that f16 cannot hold is scaled to [2^13, 2^14).  Small ones need
         // no scale: what their low parts lose below f16's range is 2^-25 of a
         // score, an absolute error.
         const int e = (int)((__float_as_uint(mx) >> 23) & 255u);
         const int ue = e >= 127 + 14 && e < 255 ? 140 + 127 - e : 127;
         const float up = a.qscale * __uint_as_float((uint32_t)ue << 23);
-        inv = __shfl(__uint_as_float((uint32_t)(254 - ue) << 23), n << 2);  // column n's
+        inv = __uint_as_float((uint32_t)(254 - ue) << 23);
 #pragma unroll
-        for (int i = 0; i < E; ++i) rows[mine][l4 * E + i] = y[i] * up;
-        __asm__ volatile("" ::: "memory");  // a wave's LDS accesses run in order
+        for (int b = 0; b < NB; ++b) y[b] *= up;
       }
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         uint32_t h[4], l[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float x = rows[n][32 * s + 8 * g + 2 * j], y = rows[n][32 * s + 8 * g + 2 * j + 1];
-          h[j] = pk_f16(x, y);
-          l[j] = NH == 2 ? pk_f16(f16_rest(x, h[j], 0), f16_rest(y, h[j], 1)) : 0u;
+          const float v0 = y[2 * s + (j >> 1)][2 * (j & 1)], v1 = y[2 * s + (j >> 1)][2 * (j & 1) + 1];
+          h[j] = pk_f16(v0, v1);
+          l[j] = NH == 2 ? pk_f16(f16_rest(v0, h[j], 0), f16_rest(v1, h[j], 1)) : 0u;
         }
         qh[ct][s] = __builtin_bit_cast(half8, u32x4{h[0], h[1], h[2], h[3]});
         if constexpr (NH == 2) ql[ct][s] = __builtin_bit_cast(half8, u32x4{l[0], l[1], l[2], l[3]});
       }
-      __asm__ volatile("" ::: "memory");
       qs[ct] = inv;
       qlarge |= __builtin_amdgcn_ballot_w64(inv != 1.f) != 0 ? 1 : 0;
     }

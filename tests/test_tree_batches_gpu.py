@@ -128,3 +128,18 @@ def test_step_tables_at_the_end_of_int32(cuda, listed):
     assert got.missing.tolist() == [lacked]
     if listed:
         assert kw["num_blocks"].tolist() == [4, 1, 4] and kw["free_count"].tolist() == [1]
+
+
+@pytest.mark.parametrize("q_type,out_type", [(torch.float32, torch.bfloat16), (torch.float32, torch.float16),
+                                             (torch.bfloat16, torch.float32), (torch.float16, torch.float32),
+                                             (torch.bfloat16, torch.float16), (torch.float16, torch.bfloat16)])
+@pytest.mark.parametrize("d,kb,vb,kind", [(64, 4, 4, "rht"), (128, 3, 2, "rht"), (256, 2, 4, "rht"), (128, 8, 8, "rht"),
+                                          (128, RAW, RAW, "rht"), (64, 3, 3, "planar"), (256, 4, 4, "iso_full")])
+def test_query_and_output_types(cuda, d, kb, vb, kind, q_type, out_type):
+    c = Case(cuda, d, kb, vb, 1, 4, [70, 300], [20, 3], vrot=kb != RAW, kind=kind, seed=25)
+    q, mask = c.q.to(q_type), c.trees()
+    want, _, share = c.want(mask, q=q)
+    for splits in (1, 4):
+        out = torch.empty(c.T, 4, d, dtype=out_type, device=cuda)
+        assert c.run(mask, q=q, out=out, num_splits=splits) is out
+        assert _rel(out.float(), want) < (1e-5 if out_type == torch.float32 else HALF[out_type] + share)

@@ -12,8 +12,9 @@
 //      place (mantissa bits, one packed multiply-add), written as the four
 //      positions of each dim, the transposition that the product needs
 // Measured steps, 16 sequences of 1024-6000 positions, up to 32 nodes, 128-wide heads
-// (us): through rows of LDS 580, this scheme 94, parts of one length 75, four lanes a
-// query 71, and the table's scale searched by four waves 70.  Measured and not kept:
+// (us): through rows of LDS 580, this scheme 94, parts of one length 75, the table's
+// scale searched by four waves and the queries four lanes each 70, their transform as a
+// matrix product 67.  Measured and not kept:
 // vector and matrix instructions interleaved by hand (98000 positions: 340 -> 362 us),
 // wave priorities around the products (340 -> 344).
 // Operands: K table values as f16 (a common scale that keeps their relative

@@ -23,12 +23,12 @@
 //
 // Cost: a tile of 32 positions takes a wave some 230 vector and 36 matrix
 // instructions at 32 columns of 128 dims, and 20 KB of LDS reads.  Two conversations of
-// 98000 positions with 61 nodes of 32 heads, K4 V2: 397 us with the merge, 197 GFLOP at
-// 497 TFLOP/s; vector units busy 58% of the time, matrix units 28%, LDS 38%, at two
+// 98000 positions with 61 nodes of 32 heads, K4 V2: 390 us with the merge, 197 GFLOP at
+// 504 TFLOP/s; vector units busy 58% of the time, matrix units 28%, LDS 38%, at two
 // waves a SIMD (registers).  At 16 sequences of 1024-6000 positions with up to 32 nodes
-// 70 us, of which a workgroup's start (its share, the queries' transform, the first
-// bytes) is a seventh and the merge 5 us; at few columns (24 chains of 5 tokens, 64-wide
-// heads: 46 us, 990 GB/s) the latency of start and tile bound it.
+// 67 us, of which a workgroup's start (its share, the queries' transform, the first
+// bytes) is a tenth and the merge 5 us; at few columns (24 chains of 5 tokens, 64-wide
+// heads: 48 us, 958 GB/s) the latency of start and tile bound it.
 //
 // Operands in LDS, in the order in which lane (m, g) (m = lane & 15, g = lane >> 4)
 // reads its 16 bytes:

@@ -5,6 +5,7 @@
 // are the ones libfused_tq.so holds.  Schemas mark the tensors an operator
 // writes in place (Tensor(a!)); shape-only fake implementations for tracing
 // are registered from Python (fused_turboquant/_ops.py).
+#include <algorithm>
 #include <torch/library.h>
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -439,13 +440,19 @@ void commit_slots(at::TensorList kv_caches, const at::Tensor& block_table, const
   if (kv_caches.empty()) return;
   const at::Tensor& c0 = kv_caches[0];
   std::vector<uint8_t*> ptrs;
+  ptrs.reserve(kv_caches.size());
   for (const at::Tensor& c : kv_caches) {
-    on_device(c, "kv_cache");
-    TORCH_CHECK(c.dim() == 4 && c.scalar_type() == at::kByte && c.stride(3) == 1 && c.sizes() == c0.sizes() &&
-                    c.strides() == c0.strides() && c.device() == block_table.device(),
-                "fused_tq: kv_caches must be uint8 [num_blocks, block_size, Hkv, slot] of one shape, layout and device");
+    TORCH_CHECK_VALUE(c.scalar_type() == at::kByte && c.dim() == 4,
+                      "fused_tq: kv_caches must be uint8 [num_blocks, block_size, num_kv_heads, slot]");
+    TORCH_CHECK_VALUE(c.stride(3) == 1, "fused_tq: kv_cache slot bytes must be contiguous");
+    TORCH_CHECK_VALUE(c.sizes() == c0.sizes() && c.strides() == c0.strides() && c.device() == block_table.device(),
+                      "fused_tq: kv_caches must have one shape and layout, on one device");
     ptrs.push_back(c.data_ptr<uint8_t>());
   }
+  std::vector<uint8_t*> sorted(ptrs);
+  std::sort(sorted.begin(), sorted.end());
+  TORCH_CHECK_VALUE(c0.numel() == 0 || std::adjacent_find(sorted.begin(), sorted.end()) == sorted.end(),
+                    "fused_tq: kv_caches names a cache twice");
   const int64_t B = block_table.dim() == 2 ? block_table.size(0) : -1;
   TORCH_CHECK(B >= 0 && block_table.scalar_type() == at::kInt && past_lens.scalar_type() == at::kInt &&
                   path.scalar_type() == at::kInt && counts.scalar_type() == at::kInt && past_lens.numel() == B &&

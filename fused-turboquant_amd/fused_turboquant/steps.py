@@ -158,6 +158,19 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, targets: torch.Tens
     return Accepted(*_ops.ops().tree_accept(tok, par, tgt, qsl, int(max_nodes)))
 
 
+def _check_caches(caches: Sequence[torch.Tensor]) -> None:
+    first = caches[0]
+    for c in caches:
+        if c.dtype != torch.uint8 or c.dim() != 4:
+            raise ValueError("kv_caches must be uint8 [num_blocks, block_size, num_kv_heads, slot]")
+        if c.stride(3) != 1:
+            raise ValueError("kv_cache slot bytes must be contiguous")
+        if c.shape != first.shape or c.stride() != first.stride() or c.device != first.device:
+            raise ValueError("kv_caches must have one shape and layout, on one device")
+    if len({c.data_ptr() for c in caches}) != len(caches):
+        raise ValueError("kv_caches names a cache twice")
+
+
 def commit_slots(kv_caches: Sequence[torch.Tensor], block_table: torch.Tensor, past_lens: torch.Tensor,
                  path: torch.Tensor, counts: torch.Tensor) -> None:
     """Move the slots of every accepted path together, in place: in each cache
@@ -181,20 +194,7 @@ def commit_slots(kv_caches: Sequence[torch.Tensor], block_table: torch.Tensor, p
         raise ValueError("past_lens, counts and path must have one entry (row) per row of block_table")
     if not caches:
         return
-    first = caches[0]
-    if first.dim() != 4:
-        raise ValueError("kv_caches must be uint8 [num_blocks, block_size, num_kv_heads, slot]")
-    shape, stride, device = first.shape, first.stride(), first.device
-    if stride[3] != 1:
-        raise ValueError("kv_cache slot bytes must be contiguous")
-    seen = set()
-    for c in caches:  # (once per layer and step: few calls each)
-        if c.dtype != torch.uint8:
-            raise ValueError("kv_caches must be uint8 [num_blocks, block_size, num_kv_heads, slot]")
-        if c.shape != shape or c.stride() != stride or c.device != device:
-            raise ValueError("kv_caches must have one shape and layout, on one device")
-        seen.add(c.data_ptr())
-    if len(seen) != len(caches):
-        raise ValueError("kv_caches names a cache twice")
-    _lib.require_device(first, block_table, past, pth, cnt)
+    if not caches[0].is_cuda:  # (the operator checks the layers' caches, in less time)
+        _check_caches(caches)
+    _lib.require_device(caches[0], block_table, past, pth, cnt)
     _ops.ops().commit_slots(caches, block_table.contiguous(), past, pth, cnt)

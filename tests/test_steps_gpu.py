@@ -305,3 +305,20 @@ def test_accept_and_commit_refusals():
             steps.commit_slots(*args)
     with pytest.raises(_lib.FusedTQError):
         steps.commit_slots([c], bt, past, path, cnt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spoil,match", [
+    (lambda c: [c[0], c[0]], "twice"), (lambda c: [c[0], c[1][:3]], "one shape"), (lambda c: [c[0], c[1].int()], "uint8"),
+    (lambda c: [c[0], c[1].transpose(1, 2)], "one shape"), (lambda c: [c[0], c[1].cpu()], "one device"),
+    (lambda c: [c[0][0], c[1]], "uint8"), (lambda c: [c[0][..., ::2], c[1][..., ::2]], "contiguous")])
+def test_commit_refuses_caches_on_the_device(cuda, spoil, match):
+    from fused_turboquant import steps
+    caches = [torch.randint(0, 256, (4, 16, 16, 64), dtype=torch.uint8, device=cuda) for _ in range(2)]
+    was = [c.clone() for c in caches]
+    i32 = dict(dtype=I32, device=cuda)
+    args = (torch.zeros(1, 4, **i32), torch.zeros(1, **i32), torch.tensor([[0, 2, 3]], **i32), torch.full((1,), 3, **i32))
+    with pytest.raises(ValueError, match=match):
+        steps.commit_slots(spoil(caches), *args)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(caches, was))

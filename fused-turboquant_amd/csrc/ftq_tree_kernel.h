@@ -543,22 +543,28 @@ struct TreeWave {
         }
         float mx = 0.f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b) {
+          // (the compiler knows what to wait for before this product reads a matrix
+          // instruction's result; before inline assembly it does not)
+          y[b] *= a.qscale;
 #pragma unroll
           for (int i = 0; i < 4; i += 2) {
             const float v0 = y[b][i], v1 = y[b][i + 1];
             asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(mx) : "v"(v0), "v"(v1));
           }
-        mx = warp_max_q(mx) * fabsf(a.qscale);
+        }
+        mx = warp_max_q(mx);
         // A query that f16 cannot hold is scaled to [2^13, 2^14).  Small ones need
         // no scale: what their low parts lose below f16's range is 2^-25 of a
         // score, an absolute error.
         const int e = (int)((__float_as_uint(mx) >> 23) & 255u);
         const int ue = e >= 127 + 14 && e < 255 ? 140 + 127 - e : 127;
-        const float up = a.qscale * __uint_as_float((uint32_t)ue << 23);
         inv = __uint_as_float((uint32_t)(254 - ue) << 23);
+        if (__builtin_amdgcn_ballot_w64(ue != 127) != 0) {
+          qlarge = 1;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) y[b] *= up;
+          for (int b = 0; b < NB; ++b) y[b] *= __uint_as_float((uint32_t)ue << 23);
+        }
       }
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
@@ -573,7 +579,6 @@ struct TreeWave {
         if constexpr (NH == 2) ql[ct][s] = __builtin_bit_cast(half8, u32x4{l[0], l[1], l[2], l[3]});
       }
       qs[ct] = inv;
-      qlarge |= __builtin_amdgcn_ballot_w64(inv != 1.f) != 0 ? 1 : 0;
     }
   }
 

@@ -143,3 +143,20 @@ def test_query_and_output_types(cuda, d, kb, vb, kind, q_type, out_type):
         out = torch.empty(c.T, 4, d, dtype=out_type, device=cuda)
         assert c.run(mask, q=q, out=out, num_splits=splits) is out
         assert _rel(out.float(), want) < (1e-5 if out_type == torch.float32 else HALF[out_type] + share)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,kb,vb", [(64, 4, 4), (128, 2, 2), (256, 3, 4), (64, RAW, RAW), (128, 8, 8)])
+def test_queries_beyond_f16(cuda, d, kb, vb, dtype):
+    """Rows that f16 cannot hold are scaled for the products; the others stay what they were."""
+    c = Case(cuda, d, kb, vb, 1, 4, [50], [20], seed=26)
+    q = c.q.to(dtype)
+    want = c.run(q=q)
+    odd = q.clone()
+    for row, head in ((0, 0), (3, 1), (19, 3)):  # a column of several waves
+        odd[row, head] *= 1e6
+    got = c.run(q=odd)
+    assert torch.isfinite(got).all()
+    for row, head in ((0, 0), (3, 1), (19, 3)):
+        got[row, head] = want[row, head]
+    assert _rel(got.float(), want.double().cpu().numpy()) < 1e-6
